@@ -33,6 +33,7 @@ extern "C" {
 #define LS_ERR_UNSUPPORTED (-6)
 #define LS_ERR_SCRATCH_TOO_SMALL (-7)
 #define LS_ERR_NOALLOC_LIMIT (-8) /* ls_paged_decode_fp16_noalloc: shape past its fixed scratch */
+#define LS_ERR_OVERLAP (-9)       /* ls_copy_pages: a page written twice, or both read and written */
 #define LS_NOALLOC_SCRATCH_BYTES 4264704
 
 /* `flags` of the decode entry points. The low byte of ls_paged_decode_fp16's
@@ -461,6 +462,78 @@ int ls_qkv_rope_append_fp16(const void* x, const void* gamma, const float* sumsq
                             int mode, float eps, int64_t max_pos, int64_t num_slots, int64_t sx,
                             int64_t sw, int64_t s_cos, int64_t sq_b, int64_t sp_t, int64_t sp_h,
                             int64_t sb_b, int64_t sb_h, void* stream);
+
+/* ---- A KV cache held in 4 bits (no counterpart in the reference) ----
+ *
+ * One pool per layer: everything a page of 16 tokens holds of one KV head is one record of
+ * 2048 + 128 * groups bytes (csrc/int4_page.cuh), `groups` = 4, 2 or 1 scales per row of 128
+ * channels (one per 32, 64 or 128). A value stands for lo + step * code, code 0..15, lo and step
+ * fp16. kv_pool [NB, H] records, strides sp_b, sp_h in BYTES (multiples of 16).
+ *
+ * Decode attention, as ls_paged_decode_fp16 (same scratch and partitioning; sized for 3 resident
+ * CTAs per SM). flags: LS_LAUNCH_PROGRAMMATIC, LS_EARLY_PAGES (only a sequence's last page is
+ * written between two steps). */
+int ls_paged_decode_int4(const void* q, const void* kv_pool, const int32_t* block_tables, const int32_t* seq_lens,
+                         float* part_acc, float* part_m, float* part_l, int32_t* seg_range, void* out, int batch,
+                         int kv_heads, int n_rep, int groups, int head_dim, int page, int max_pages, int num_blocks,
+                         int num_chunks, int min_chunk, int flags, int64_t sq_b, int64_t sq_h, int64_t sq_m,
+                         int64_t sp_b, int64_t sp_h, int64_t so_b, int64_t so_h, int64_t so_m, float softmax_scale,
+                         void* stream);
+
+/* Quantise new rows k, v fp16 [B, H, tokens, 128] (strides sk_*, sv_*; 16-byte aligned) into the
+ * pages: rows 0 .. m-1 of sequence b go to positions seq_lens[b] - m .. seq_lens[b] - 1,
+ * m = min(new_lens[b], tokens), or tokens where new_lens is NULL. step = fp16((max - lo) / 15),
+ * code = rne((x - lo) / step), NaN as 0, infinities as the largest fp16. Positions below zero, past
+ * max_pages or in a block outside the pool are dropped. No byte of another token is written. */
+int ls_int4_write(const void* k, const void* v, void* kv_pool, const int32_t* block_tables, const int32_t* seq_lens,
+                  const int32_t* new_lens, int batch, int kv_heads, int tokens, int groups, int head_dim, int page,
+                  int max_pages, int num_blocks, int64_t sk_b, int64_t sk_h, int64_t sk_t, int64_t sv_b, int64_t sv_h,
+                  int64_t sv_t, int64_t sp_b, int64_t sp_h, void* stream);
+
+/* The values of positions start[b] .. start[b] + tokens - 1 (start NULL: 0) into k, v fp16
+ * [B, H, tokens, 128]; zeros at and past seq_lens[b] and for blocks outside the pool. */
+int ls_int4_read(const void* kv_pool, void* k, void* v, const int32_t* block_tables, const int32_t* seq_lens,
+                 const int32_t* start, int batch, int kv_heads, int tokens, int groups, int head_dim, int page,
+                 int max_pages, int num_blocks, int64_t sk_b, int64_t sk_h, int64_t sk_t, int64_t sv_b, int64_t sv_h,
+                 int64_t sv_t, int64_t sp_b, int64_t sp_h, void* stream);
+
+/* ls_rope_append_fp16 for the 4-bit cache: q rotated into q_out, rotated k and v quantised into
+ * the page of flat slot slots[b]. */
+int ls_rope_append_int4(const void* qkv, const void* cos, const void* sin, const int64_t* positions,
+                        const int64_t* slots, void* q_out, void* kv_pool, int batch, int q_heads, int kv_heads,
+                        int groups, int head_dim, int page, int64_t max_pos, int64_t num_blocks, int64_t s_qkv,
+                        int64_t s_cos, int64_t sq_b, int64_t sp_b, int64_t sp_h, void* stream);
+
+/* ---- Pages of any cache ----
+ *
+ * One kind of pool, `layers` times: page i of layer l starts layer_stride * l + page_stride * i
+ * bytes behind base and is page_bytes long. */
+typedef struct {
+    void* base;
+    int64_t layer_stride, page_stride; /* bytes */
+    int32_t page_bytes, layers;
+} ls_page_pool;
+
+/* page dst[i] = page src[i], i < count, in every pool and layer. pools, src and dst are HOST
+ * arrays, read before the call returns (a captured launch keeps its ids). One launch per 64 pools
+ * and 3584 pages. A page may be read many times; one that is written twice, or both read and
+ * written, is refused (LS_ERR_OVERLAP). */
+int ls_copy_pages(const ls_page_pool* pools, int num_pools, const int32_t* src, const int32_t* dst, int count,
+                  int num_blocks, void* stream);
+
+/* ---- Rotary positions ----
+ *
+ * q [tokens, q_heads, dim] and k [tokens, k_heads, dim] rotated by their positions into q_out and
+ * k_out (which may be q and k themselves). Strides s?_t, s?_h in elements, channels dense. The first
+ * `rot` channels turn, pairs (i, i + rot/2) or with `interleaved` (2i, 2i+1); the others are copied.
+ * cos, sin fp32 [max_pos, rot/2] (row stride s_tab). dtype 0 fp16, 1 bf16, 2 fp32; fp32 arithmetic,
+ * one rounding. `inverse` turns back: the gradient of the forward. A position outside the
+ * tables gives NaN in the rotated channels. q_heads or k_heads may be 0.
+ * The reference has the half layout over the whole head, `rope_qk` (kernels/fused_elementwise.py:229-252). */
+int ls_rotary(const void* q, const void* k, void* q_out, void* k_out, const float* cos, const float* sin,
+              const int64_t* positions, int tokens, int q_heads, int k_heads, int dim, int rot, int dtype,
+              int interleaved, int inverse, int64_t max_pos, int64_t s_tab, int64_t sq_t, int64_t sq_h, int64_t sk_t,
+              int64_t sk_h, int64_t sqo_t, int64_t sqo_h, int64_t sko_t, int64_t sko_h, void* stream);
 
 #ifdef __cplusplus
 }

@@ -31,6 +31,7 @@ STATUS = {
     -7: "scratch buffer too small",
     -8: "shape past the fixed scratch of the allocation-free entry point "
         "(needs batch <= 64 and (batch + num_chunks) * kv_heads <= 1024)",
+    -9: "a page is written twice, or both read and written",
 }
 
 P, I, L, F = c_void_p, c_int, c_int64, c_float
@@ -59,6 +60,12 @@ _PROTOTYPES = {
     "ls_rope_append_fp16": [P] * 10 + [I] * 5 + [L] * 9 + [P],
     "ls_skinny_gemm": [P] * 5 + [I] + [P] * 7 + [I] * 5 + [F] + [L] * 6 + [P],
     "ls_rope_append_int8": [P] * 13 + [I] * 4 + [L] * 8 + [I] + [F] * 6 + [P],
+    "ls_paged_decode_int4": [P] * 9 + [I] * 11 + [L] * 8 + [F, P],
+    "ls_int4_write": [P] * 6 + [I] * 8 + [L] * 8 + [P],
+    "ls_int4_read": [P] * 6 + [I] * 8 + [L] * 8 + [P],
+    "ls_rope_append_int4": [P] * 7 + [I] * 6 + [L] * 7 + [P],
+    "ls_copy_pages": [P, I, P, P, I, I, P],
+    "ls_rotary": [P] * 7 + [I] * 8 + [L] * 10 + [P],
     "ls_qkv_rope_append_fp16": [P] * 3 + [I] + [P] * 13 + [I] * 8 + [F] + [L] * 10 + [P],
 }
 

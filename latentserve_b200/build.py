@@ -23,7 +23,8 @@ CSRC = HERE / "csrc"
 OUT_DIR = HERE / "_C"
 LIB = OUT_DIR / "libls_b200.so"
 SOURCES = ("paged_decode.cu", "kv_write.cu", "page_select.cu", "fused_elementwise.cu",
-           "skinny_gemm.cu")
+           "skinny_gemm.cu", "int4_write.cu", "paged_decode_int4.cu",
+           "page_copy.cu", "rotary.cu")
 ARCH_FLAGS = ("-gencode", "arch=compute_100a,code=sm_100a")
 
 
@@ -42,7 +43,7 @@ def needs_build() -> bool:
     if not LIB.exists():
         return True
     built = LIB.stat().st_mtime
-    deps = list(CSRC.glob("*.cu")) + list(CSRC.glob("*.cuh"))
+    deps = [*CSRC.glob("*.cu"), *CSRC.glob("*.cuh"), *HERE.parent.glob("include/*.h")]
     return any(p.stat().st_mtime > built for p in deps)
 
 

@@ -40,6 +40,7 @@ from latentserve_b200 import fused_elementwise as fe
 from latentserve_b200 import paged_decode as pd
 from latentserve_b200 import paged_sparse as ps
 from latentserve_b200 import projections as pj
+from latentserve_b200 import rotary
 
 
 @dataclass
@@ -54,6 +55,7 @@ class QwenShape:
     vocab: int = 151936
     rms_eps: float = 1e-6
     rope_theta: float = 1e6
+    rope_scaling: Optional[dict] = None        # for contexts past the trained ones, see `rotary`
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:
@@ -63,6 +65,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:
 
 def rope_tables(shape: QwenShape, max_pos: int, device) -> tuple[torch.Tensor, torch.Tensor]:
     """cos / sin [max_pos, head_dim], halves duplicated (rotate-half convention)."""
+    if shape.rope_scaling is not None:
+        cos, sin = rotary.rotary_tables(shape.head_dim, max_pos, shape.rope_theta, shape.rope_scaling, device)
+        return torch.cat([cos, cos], dim=-1), torch.cat([sin, sin], dim=-1)
     half = shape.head_dim // 2
     inv = shape.rope_theta ** (-torch.arange(half, dtype=torch.float32, device=device) / half)
     ang = torch.arange(max_pos, dtype=torch.float32, device=device)[:, None] * inv[None, :]
@@ -120,6 +125,8 @@ class DecodeModel:
 
     def attend(self, cache, layer: int, q: torch.Tensor, batch: int, context_hint: int) -> torch.Tensor:
         tables, lens = cache.block_tables_tensor(batch), cache.seq_lens_tensor(batch)
+        if hasattr(cache, "kv_pool"):                        # 4-bit cache
+            return pd.paged_decode_attention_int4(q, cache.kv_pool[layer], tables, lens, workspace=cache.workspace)
         extra = {}
         if hasattr(cache, "k_scale_pool"):
             extra = dict(k_scale=cache.k_scale_pool[layer], v_scale=cache.v_scale_pool[layer],

@@ -100,6 +100,27 @@ def paged_decode_attention(
     return out
 
 
+def paged_decode_attention_int4(
+    q: torch.Tensor,
+    kv_pool: torch.Tensor,
+    block_tables: torch.Tensor,
+    seq_lens: torch.Tensor,
+    softmax_scale: Optional[float] = None,
+    max_seq_len: Optional[int] = None,
+    out: Optional[torch.Tensor] = None,
+    workspace: Optional[pdc.DecodeWorkspace] = None,
+) -> torch.Tensor:
+    """`paged_decode_attention` over a cache held in 4 bits: kv_pool [num_blocks, H_kv, record]
+    uint8, one record per page and KV head (`int4_write`, `cache.Int4PagedKVCache.kv_pool`).
+
+    No counterpart in the reference (its pools are fp16 or INT8). `max_seq_len` is accepted for
+    symmetry and ignored. The result is a tensor of its own unless `out` is given. `workspace`
+    names the bookkeeping buffers to use (see `paged_decode_cuda.DecodeWorkspace`); by default
+    calls of one stream share theirs and every captured call has its own.
+    """
+    return pdc.paged_decode_int4(q, kv_pool, block_tables, seq_lens, softmax_scale, out, workspace)
+
+
 _PLANS: dict = {}
 _PLAN_LIMIT = 4096
 # k_pool address -> (k_new, v_new) of a cache.write() whose append was left to the next

@@ -43,6 +43,8 @@ MIN_CHUNK_PAGES = 8                 # never cut the page axis finer than this
 CTAS_PER_SM = 2                     # resident CTAs per SM the kernels are sized for
 # ... and for the INT8 kernel (must match LS_INT8_CTAS the library was built with)
 INT8_CTAS_PER_SM = int(os.environ.get("LATENTSERVE_B200_INT8_CTAS", "3"))
+# ... and for the 4-bit kernel (must match LS_INT4_CTAS in csrc/paged_decode_int4.cu)
+INT4_CTAS_PER_SM = 3
 MAX_BATCH = 1024
 
 _SCRATCH: dict = {}
@@ -299,3 +301,91 @@ def plan_decode(q, k_pool, v_pool, block_tables, seq_lens, num_splits=None, soft
             k_pool.stride(0), k_pool.stride(1), k_pool.stride(2),
             out.stride(0), out.stride(1), out.stride(2), scale)
     return fn, args, out, dev_index
+
+
+class DecodeWorkspace:
+    """The bookkeeping of 4-bit decode launches that follow one another on the GPU: per
+    (batch, KV heads) an int32 buffer whose arrival counters every launch leaves at zero.
+    Launches that may overlap -- on two streams, in two captured graphs -- need one each. A
+    cache owns one for its own decode steps; calls without one get one per stream."""
+
+    def __init__(self):
+        self._segs: dict = {}
+
+    def seg(self, batch: int, kv_heads: int, device) -> torch.Tensor:
+        key = (batch, kv_heads, str(device))
+        buf = self._segs.get(key)
+        if buf is None:
+            buf = torch.zeros(seg_len(batch, kv_heads), dtype=torch.int32, device=device)
+            # Made while a graph is being captured, the buffer belongs to that graph, which
+            # zeroes it at every replay: not for anyone else.
+            if not torch.cuda.is_current_stream_capturing():
+                self._segs[key] = buf
+        return buf
+
+    def error_flag(self, device, batch: int, kv_heads: int) -> int:
+        """As `error_flag` above, for launches that used this workspace."""
+        buf = self._segs.get((batch, kv_heads, str(torch.device(device))))
+        return 0 if buf is None else int(buf[2 * batch].item())
+
+
+_STREAM_WORKSPACES: dict = {}
+
+
+def stream_workspace(device_index: int, stream: int) -> DecodeWorkspace:
+    """The workspace of calls that bring none: one per stream, where launches are ordered; a
+    fresh one under capture, since a graph may be replayed on any stream."""
+    if torch.cuda.is_current_stream_capturing():
+        return DecodeWorkspace()
+    return _STREAM_WORKSPACES.setdefault((device_index, stream), DecodeWorkspace())
+
+
+def int4_eligible(q: torch.Tensor, kv_pool: torch.Tensor) -> bool:
+    """What the 4-bit kernel handles: fp16 queries, head_dim 128, at most 8 query rows per KV
+    head, one uint8 pool of page records, 16-byte aligned rows."""
+    from latentserve_b200 import int4_write as i4
+
+    return (q.is_cuda and q.dtype == torch.float16 and q.dim() == 4 and q.shape[-1] == 128
+            and 1 <= q.shape[2] <= ROWS_PER_PARTIAL and 1 <= q.shape[0] <= MAX_BATCH and _aligned(q, 16)
+            and i4.pool_ok(kv_pool) and kv_pool.shape[1] == q.shape[1])
+
+
+def paged_decode_int4(q, kv_pool, block_tables, seq_lens, softmax_scale: Optional[float] = None,
+                      out: Optional[torch.Tensor] = None,
+                      workspace: Optional[DecodeWorkspace] = None) -> torch.Tensor:
+    """q [B, H_kv, N_REP, 128] fp16; kv_pool [num_blocks, H_kv, record] uint8 (see
+    `int4_write`); block_tables [B, max_pages], seq_lens [B] int32 -> [B, H_kv, N_REP, 128] fp16."""
+    from latentserve_b200 import int4_write as i4
+
+    if not q.is_cuda:
+        raise RuntimeError("latentserve_b200 has no CPU path: tensors must be on a CUDA device")
+    if not int4_eligible(q, kv_pool):
+        raise ValueError(
+            "layout not supported by the sm_100a kernels: need fp16 q with head_dim 128, <= 8 query rows per KV "
+            "head, 1 to 1024 sequences and a uint8 pool of 4-bit page records with 16-byte aligned rows")
+    b, h, r, d = q.shape
+    block_tables = i4.check_tables(block_tables, seq_lens, b, q.device)
+    if kv_pool.device != q.device:
+        raise ValueError("q and the pool must be on one device")
+    if out is None:
+        out = torch.empty((b, h, r, d), dtype=q.dtype, device=q.device)
+    elif (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.data_ptr() % 8
+          or out.stride(-1) != 1 or any(st % 4 for st in out.stride()[:-1])):
+        raise ValueError("out must be an fp16 [B, H_kv, N_REP, 128] tensor on q's device with 8-byte aligned "
+                         "rows of unit-stride channels")
+    dev_index = q.device.index
+    stream = _lib.raw_stream(dev_index)
+    chunks = choose_chunks(q.device, h, None, b, INT4_CTAS_PER_SM)
+    # Partial states: accumulators, then maxima, then sums (one allocation).
+    rows = (b + chunks) * h * ROWS_PER_PARTIAL
+    part = torch.empty(rows * 130, dtype=torch.float32, device=q.device)
+    acc = part.data_ptr()
+    seg = (workspace or stream_workspace(dev_index, stream)).seg(b, h, q.device)
+    sq, so, sp = q.stride(), out.stride(), kv_pool.stride()
+    rc = _lib.lib().ls_paged_decode_int4(
+        q.data_ptr(), kv_pool.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(), acc, acc + rows * 512,
+        acc + rows * 516, seg.data_ptr(), out.data_ptr(), b, h, r, i4.groups_of(kv_pool), d, 16,
+        block_tables.shape[1], kv_pool.shape[0], chunks, MIN_CHUNK_PAGES, dense_launch_flags(), sq[0], sq[1], sq[2],
+        sp[0], sp[1], so[0], so[1], so[2], softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(d), stream)
+    _lib.check(rc, "paged_decode_int4")
+    return out
