@@ -34,6 +34,7 @@ extern "C" {
 #define LS_ERR_SCRATCH_TOO_SMALL (-7)
 #define LS_ERR_NOALLOC_LIMIT (-8) /* ls_paged_decode_fp16_noalloc: shape past its fixed scratch */
 #define LS_ERR_OVERLAP (-9)       /* ls_copy_pages: a page written twice, or both read and written */
+#define LS_ERR_PAGE_ID (-10)      /* ls_copy_pages: a page id outside the pool */
 #define LS_NOALLOC_SCRATCH_BYTES 4264704
 
 /* `flags` of the decode entry points. The low byte of ls_paged_decode_fp16's
@@ -470,15 +471,16 @@ int ls_qkv_rope_append_fp16(const void* x, const void* gamma, const float* sumsq
  * channels (one per 32, 64 or 128). A value stands for lo + step * code, code 0..15, lo and step
  * fp16. kv_pool [NB, H] records, strides sp_b, sp_h in BYTES (multiples of 16).
  *
- * Decode attention, as ls_paged_decode_fp16 (same scratch and partitioning; sized for 3 resident
- * CTAs per SM). flags: LS_LAUNCH_PROGRAMMATIC, LS_EARLY_PAGES (only a sequence's last page is
- * written between two steps). */
+ * Decode attention, as ls_paged_decode_fp16 with `out` required. Scratch: `part` float
+ * [H * (B + num_chunks) * 1040], 16-byte aligned, never filled; `seg_range` as above, of which
+ * [0, 2B) stays unused: ZERO IT ONCE. Sized for 2 resident CTAs per SM (num_chunks = 2 * SMs / H);
+ * `min_chunk` is the fewest pages a CTA takes of a sequence that has them. flags:
+ * LS_LAUNCH_PROGRAMMATIC, LS_EARLY_PAGES (only a sequence's last page is written between two steps). */
 int ls_paged_decode_int4(const void* q, const void* kv_pool, const int32_t* block_tables, const int32_t* seq_lens,
-                         float* part_acc, float* part_m, float* part_l, int32_t* seg_range, void* out, int batch,
-                         int kv_heads, int n_rep, int groups, int head_dim, int page, int max_pages, int num_blocks,
-                         int num_chunks, int min_chunk, int flags, int64_t sq_b, int64_t sq_h, int64_t sq_m,
-                         int64_t sp_b, int64_t sp_h, int64_t so_b, int64_t so_h, int64_t so_m, float softmax_scale,
-                         void* stream);
+                         float* part, int32_t* seg_range, void* out, int batch, int kv_heads, int n_rep, int groups,
+                         int head_dim, int page, int max_pages, int num_blocks, int num_chunks, int min_chunk, int flags,
+                         int64_t sq_b, int64_t sq_h, int64_t sq_m, int64_t sp_b, int64_t sp_h, int64_t so_b,
+                         int64_t so_h, int64_t so_m, float softmax_scale, void* stream);
 
 /* Quantise new rows k, v fp16 [B, H, tokens, 128] (strides sk_*, sv_*; 16-byte aligned) into the
  * pages: rows 0 .. m-1 of sequence b go to positions seq_lens[b] - m .. seq_lens[b] - 1,

@@ -32,6 +32,7 @@ STATUS = {
     -8: "shape past the fixed scratch of the allocation-free entry point "
         "(needs batch <= 64 and (batch + num_chunks) * kv_heads <= 1024)",
     -9: "a page is written twice, or both read and written",
+    -10: "a page id lies outside the pool",
 }
 
 P, I, L, F = c_void_p, c_int, c_int64, c_float
@@ -60,7 +61,7 @@ _PROTOTYPES = {
     "ls_rope_append_fp16": [P] * 10 + [I] * 5 + [L] * 9 + [P],
     "ls_skinny_gemm": [P] * 5 + [I] + [P] * 7 + [I] * 5 + [F] + [L] * 6 + [P],
     "ls_rope_append_int8": [P] * 13 + [I] * 4 + [L] * 8 + [I] + [F] * 6 + [P],
-    "ls_paged_decode_int4": [P] * 9 + [I] * 11 + [L] * 8 + [F, P],
+    "ls_paged_decode_int4": [P] * 7 + [I] * 11 + [L] * 8 + [F, P],
     "ls_int4_write": [P] * 6 + [I] * 8 + [L] * 8 + [P],
     "ls_int4_read": [P] * 6 + [I] * 8 + [L] * 8 + [P],
     "ls_rope_append_int4": [P] * 7 + [I] * 6 + [L] * 7 + [P],
@@ -117,3 +118,36 @@ def raw_stream(device_index: int) -> int:
         raise RuntimeError(f"tensors live on cuda:{device_index} but the current device is cuda:{current}; "
                            f"call inside `with torch.cuda.device({device_index}):`")
     return torch._C._cuda_getCurrentRawStream(device_index)
+
+
+def launch_stream(device_index: int) -> int:
+    """`raw_stream` for tensors that are known to exist on a CUDA device (no lazy
+    initialisation to look after): the same check, a fraction of its cost."""
+    if torch._C._cuda_getDevice() != device_index:
+        return raw_stream(device_index)                 # says what is wrong
+    return torch._C._cuda_getCurrentRawStream(device_index)
+
+
+class Layouts:
+    """What a call works out from its tensors' layouts -- shapes, strides, types, devices -- kept
+    per layout, so that a decode loop's calls check once and launch many times. Nothing about
+    the tensors' contents or addresses is kept; alignment is checked at every call."""
+
+    def __init__(self, limit: int = 4096):
+        self._known: dict = {}
+        self._limit = limit
+
+    def get(self, key):
+        return self._known.get(key)
+
+    def put(self, key, value):
+        if len(self._known) >= self._limit:
+            self._known.clear()
+        self._known[key] = value
+        return value
+
+
+def bound(name: str, first: int, values) -> tuple:
+    """`values` as the C types of entry point `name`'s parameters from number `first` on: a call
+    that is made again and again converts only what changes."""
+    return tuple(kind(v) for kind, v in zip(_PROTOTYPES[name][first:], values, strict=False))

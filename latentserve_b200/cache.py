@@ -212,6 +212,7 @@ class _PagedBase:
         self._block_tables = self._seq_lens_tensor = self._write_slots = None
         self._prefill_slots: Optional[torch.Tensor] = None
         self._decode_slot_vec: Optional[torch.Tensor] = None      # [b] view of the decode slots
+        self._copier: Optional[tuple] = None                      # the pools' description for page copies
 
     # -- state ---------------------------------------------------------
     @property
@@ -257,8 +258,11 @@ class _PagedBase:
         """Device writes of the last step that are still to be launched."""
 
     def _copy_pages(self, src: Sequence[int], dst: Sequence[int]) -> None:
-        for tensors, block_dim in self._page_pools():
-            page_copy.copy_pages(tensors, src, dst, block_dim)
+        bounds = getattr(self, "_bounds_on", False)             # pools that came later
+        if self._copier is None or self._copier[0] != bounds:
+            self._copier = bounds, [page_copy.PagePools(tensors, dim) for tensors, dim in self._page_pools()]
+        for pools in self._copier[1]:
+            pools.copy(src, dst)
 
     def fork(self, source: int, targets: Sequence[int]) -> None:
         """Start the empty slots `targets` as copies of the sequence in slot `source` (beam

@@ -80,7 +80,7 @@ static int launch_copies(CopyArgs<PAIRS>& a, const int32_t* src, const int32_t* 
 // Every id inside the pool; no page written twice, none both read and written.
 static int check_pairs(const int32_t* src, const int32_t* dst, int count, int num_blocks) {
     for (int i = 0; i < count; ++i)
-        if (src[i] < 0 || src[i] >= num_blocks || dst[i] < 0 || dst[i] >= num_blocks) return LS_ERR_BAD_SHAPE;
+        if (src[i] < 0 || src[i] >= num_blocks || dst[i] < 0 || dst[i] >= num_blocks) return LS_ERR_PAGE_ID;
     unsigned char* written = static_cast<unsigned char*>(calloc((size_t)num_blocks / 8 + 1, 1));
     if (written == nullptr) return (int)cudaErrorMemoryAllocation;
     int rc = LS_OK;

@@ -9,9 +9,9 @@ given, all layers, one launch. The reference shares whole pages by reference cou
 from __future__ import annotations
 
 import ctypes
+from array import array
 from typing import Sequence
 
-import numpy as np
 import torch
 
 from latentserve_b200 import _lib
@@ -37,14 +37,39 @@ def _describe(t: torch.Tensor, block_dim: int) -> _Pool:
                  t.shape[0] if block_dim else 1)
 
 
-def _ids(x, what: str) -> np.ndarray:
+def _ids(x, what: str) -> array:
     """Page ids as int32, refused where they would not survive the conversion."""
-    a = np.asarray(x)
-    if a.ndim != 1 or (a.size and a.dtype.kind not in "iu"):
-        raise ValueError(f"{what} must be a flat sequence of whole numbers")
-    if a.size and (a.min() < 0 or a.max() >= 2 ** 31):
-        raise ValueError(f"{what} holds a page id outside the pool")
-    return np.ascontiguousarray(a, dtype=np.int32)
+    try:
+        return array("i", x)
+    except (TypeError, OverflowError) as e:
+        raise ValueError(f"{what} must be a flat sequence of page ids (whole numbers): {e}") from None
+
+
+class PagePools:
+    """The pools one kind of copy goes through, described once: for who copies again and again
+    (a cache). Keeps the tensors alive."""
+
+    def __init__(self, pools: Sequence[torch.Tensor], block_dim: int = 0):
+        if block_dim not in (0, 1):
+            raise ValueError("block_dim must be 0 or 1")
+        self.pools = list(pools)
+        self.table = (_Pool * len(self.pools))(*[_describe(t, block_dim) for t in self.pools])
+        self.blocks = self.pools[0].shape[block_dim] if self.pools else 0
+        self.index = self.pools[0].get_device() if self.pools else -1
+        if any(t.shape[block_dim] != self.blocks or t.get_device() != self.index for t in self.pools):
+            raise ValueError("the pools must have one number of pages, on one device")
+
+    def copy(self, src: Sequence[int], dst: Sequence[int]) -> None:
+        """pool[dst[i]] = pool[src[i]] in every pool; see `copy_pages`."""
+        s, d = _ids(src, "src"), _ids(dst, "dst")
+        if len(s) != len(d):
+            raise ValueError(f"{len(s)} source pages for {len(d)} destinations")
+        if not s or not self.pools:
+            return
+        rc = _lib.lib().ls_copy_pages(self.table, len(self.pools), s.buffer_info()[0], d.buffer_info()[0], len(s),
+                                      self.blocks, _lib.launch_stream(self.index))
+        if rc:
+            _lib.check(rc, "copy_pages")
 
 
 def copy_pages(pools: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[int], block_dim: int = 0) -> None:
@@ -53,21 +78,4 @@ def copy_pages(pools: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[
     host sequences of page ids: they are read before the call returns, and a captured call
     replays with the same ids. A source may serve several destinations; a destination given
     twice, or that is a source as well, is refused."""
-    if block_dim not in (0, 1):
-        raise ValueError("block_dim must be 0 or 1")
-    if not pools:
-        return
-    blocks, device = pools[0].shape[block_dim] if pools[0].dim() > block_dim else 0, pools[0].device
-    table = (_Pool * len(pools))(*(_describe(t, block_dim) for t in pools))
-    if any(t.shape[block_dim] != blocks or t.device != device for t in pools):
-        raise ValueError("the pools must have one number of pages, on one device")
-    s, d = _ids(src, "src"), _ids(dst, "dst")
-    if s.size != d.size:
-        raise ValueError(f"{s.size} source pages for {d.size} destinations")
-    if s.size == 0:
-        return
-    if max(int(s.max()), int(d.max())) >= blocks:
-        raise ValueError(f"a page id lies outside the pool of {blocks} pages")
-    rc = _lib.lib().ls_copy_pages(table, len(pools), s.ctypes.data, d.ctypes.data, int(s.size), blocks,
-                                  _lib.raw_stream(device.index))
-    _lib.check(rc, "copy_pages")
+    PagePools(pools, block_dim).copy(src, dst)

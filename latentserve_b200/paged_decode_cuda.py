@@ -22,6 +22,7 @@ from typing import Optional
 import torch
 
 from latentserve_b200 import _lib
+from latentserve_b200 import int4_write as i4
 
 IMPL_MMA, IMPL_SIMT = 0, 1          # tensor-core kernel / CUDA-core kernel (fp16 pools)
 LAUNCH_PROGRAMMATIC = 0x100         # see LS_LAUNCH_PROGRAMMATIC in the header
@@ -44,7 +45,8 @@ CTAS_PER_SM = 2                     # resident CTAs per SM the kernels are sized
 # ... and for the INT8 kernel (must match LS_INT8_CTAS the library was built with)
 INT8_CTAS_PER_SM = int(os.environ.get("LATENTSERVE_B200_INT8_CTAS", "3"))
 # ... and for the 4-bit kernel (must match LS_INT4_CTAS in csrc/paged_decode_int4.cu)
-INT4_CTAS_PER_SM = 3
+INT4_CTAS_PER_SM = int(os.environ.get("LATENTSERVE_B200_INT4_CTAS", "2"))
+INT4_MIN_CHUNK = 16                 # pages of a long sequence a CTA takes at least: four a warp
 MAX_BATCH = 1024
 
 _SCRATCH: dict = {}
@@ -304,29 +306,32 @@ def plan_decode(q, k_pool, v_pool, block_tables, seq_lens, num_splits=None, soft
 
 
 class DecodeWorkspace:
-    """The bookkeeping of 4-bit decode launches that follow one another on the GPU: per
-    (batch, KV heads) an int32 buffer whose arrival counters every launch leaves at zero.
-    Launches that may overlap -- on two streams, in two captured graphs -- need one each. A
-    cache owns one for its own decode steps; calls without one get one per stream."""
+    """The scratch of 4-bit decode launches that follow one another on the GPU: per (batch, KV
+    heads, partial states) the partial states and an int32 buffer whose arrival counters every
+    launch leaves at zero. Launches that may overlap -- on two streams, in two captured graphs --
+    need one each. A cache owns one for its own decode steps; calls without one get one per stream."""
 
     def __init__(self):
-        self._segs: dict = {}
+        self._held: dict = {}
 
-    def seg(self, batch: int, kv_heads: int, device) -> torch.Tensor:
-        key = (batch, kv_heads, str(device))
-        buf = self._segs.get(key)
-        if buf is None:
-            buf = torch.zeros(seg_len(batch, kv_heads), dtype=torch.int32, device=device)
-            # Made while a graph is being captured, the buffer belongs to that graph, which
-            # zeroes it at every replay: not for anyone else.
+    def get(self, batch: int, kv_heads: int, rows: int, device) -> tuple:
+        """(addresses of the partial states and the bookkeeping, the two buffers)"""
+        key = (batch, kv_heads, rows, device)
+        held = self._held.get(key)
+        if held is None:
+            part = torch.empty(rows * 130, dtype=torch.float32, device=device)
+            seg = torch.zeros(seg_len(batch, kv_heads), dtype=torch.int32, device=device)
+            held = (part.data_ptr(), seg.data_ptr()), part, seg
+            # Made while a graph is being captured, the buffers belong to that graph, which
+            # zeroes the counters at every replay: not for anyone else.
             if not torch.cuda.is_current_stream_capturing():
-                self._segs[key] = buf
-        return buf
+                self._held[key] = held
+        return held
 
     def error_flag(self, device, batch: int, kv_heads: int) -> int:
         """As `error_flag` above, for launches that used this workspace."""
-        buf = self._segs.get((batch, kv_heads, str(torch.device(device))))
-        return 0 if buf is None else int(buf[2 * batch].item())
+        return max((int(seg[2 * batch].item()) for (b, h, _, dev), (_, _, seg) in self._held.items()
+                    if (b, h, dev) == (batch, kv_heads, torch.device(device))), default=0)
 
 
 _STREAM_WORKSPACES: dict = {}
@@ -335,28 +340,27 @@ _STREAM_WORKSPACES: dict = {}
 def stream_workspace(device_index: int, stream: int) -> DecodeWorkspace:
     """The workspace of calls that bring none: one per stream, where launches are ordered; a
     fresh one under capture, since a graph may be replayed on any stream."""
-    if torch.cuda.is_current_stream_capturing():
+    if torch._C._cuda_isCurrentStreamCapturing():
         return DecodeWorkspace()
-    return _STREAM_WORKSPACES.setdefault((device_index, stream), DecodeWorkspace())
+    work = _STREAM_WORKSPACES.get((device_index, stream))
+    if work is None:
+        work = _STREAM_WORKSPACES[(device_index, stream)] = DecodeWorkspace()
+    return work
 
 
 def int4_eligible(q: torch.Tensor, kv_pool: torch.Tensor) -> bool:
     """What the 4-bit kernel handles: fp16 queries, head_dim 128, at most 8 query rows per KV
     head, one uint8 pool of page records, 16-byte aligned rows."""
-    from latentserve_b200 import int4_write as i4
-
     return (q.is_cuda and q.dtype == torch.float16 and q.dim() == 4 and q.shape[-1] == 128
-            and 1 <= q.shape[2] <= ROWS_PER_PARTIAL and 1 <= q.shape[0] <= MAX_BATCH and _aligned(q, 16)
-            and i4.pool_ok(kv_pool) and kv_pool.shape[1] == q.shape[1])
+            and 1 <= q.shape[2] <= ROWS_PER_PARTIAL and 1 <= q.shape[0] <= MAX_BATCH and q.shape[1] >= 1
+            and _aligned(q, 16) and i4.pool_ok(kv_pool) and kv_pool.shape[1] == q.shape[1])
 
 
-def paged_decode_int4(q, kv_pool, block_tables, seq_lens, softmax_scale: Optional[float] = None,
-                      out: Optional[torch.Tensor] = None,
-                      workspace: Optional[DecodeWorkspace] = None) -> torch.Tensor:
-    """q [B, H_kv, N_REP, 128] fp16; kv_pool [num_blocks, H_kv, record] uint8 (see
-    `int4_write`); block_tables [B, max_pages], seq_lens [B] int32 -> [B, H_kv, N_REP, 128] fp16."""
-    from latentserve_b200 import int4_write as i4
+_INT4_LAYOUTS = _lib.Layouts()
 
+
+def _int4_layout(key, q, kv_pool, block_tables, seq_lens, out):
+    """The arguments of a 4-bit decode launch that its tensors' layouts decide, after checking them."""
     if not q.is_cuda:
         raise RuntimeError("latentserve_b200 has no CPU path: tensors must be on a CUDA device")
     if not int4_eligible(q, kv_pool):
@@ -364,28 +368,42 @@ def paged_decode_int4(q, kv_pool, block_tables, seq_lens, softmax_scale: Optiona
             "layout not supported by the sm_100a kernels: need fp16 q with head_dim 128, <= 8 query rows per KV "
             "head, 1 to 1024 sequences and a uint8 pool of 4-bit page records with 16-byte aligned rows")
     b, h, r, d = q.shape
-    block_tables = i4.check_tables(block_tables, seq_lens, b, q.device)
+    i4.check_tables(block_tables, seq_lens, b, q.device)
     if kv_pool.device != q.device:
         raise ValueError("q and the pool must be on one device")
-    if out is None:
-        out = torch.empty((b, h, r, d), dtype=q.dtype, device=q.device)
-    elif (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.data_ptr() % 8
-          or out.stride(-1) != 1 or any(st % 4 for st in out.stride()[:-1])):
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device
+                            or out.stride(-1) != 1 or any(st % 4 for st in out.stride()[:-1])):
         raise ValueError("out must be an fp16 [B, H_kv, N_REP, 128] tensor on q's device with 8-byte aligned "
                          "rows of unit-stride channels")
-    dev_index = q.device.index
-    stream = _lib.raw_stream(dev_index)
     chunks = choose_chunks(q.device, h, None, b, INT4_CTAS_PER_SM)
-    # Partial states: accumulators, then maxima, then sums (one allocation).
     rows = (b + chunks) * h * ROWS_PER_PARTIAL
-    part = torch.empty(rows * 130, dtype=torch.float32, device=q.device)
-    acc = part.data_ptr()
-    seg = (workspace or stream_workspace(dev_index, stream)).seg(b, h, q.device)
-    sq, so, sp = q.stride(), out.stride(), kv_pool.stride()
+    counts = (b, h, r, i4.groups_of(kv_pool), d, 16, block_tables.shape[1], kv_pool.shape[0], chunks, INT4_MIN_CHUNK)
+    so = out.stride()[:3] if out is not None else (h * r * d, r * d, d)
+    name = "ls_paged_decode_int4"
+    return _INT4_LAYOUTS.put(key, ((b, h, rows, q.device), _lib.bound(name, 7, counts),
+                                   _lib.bound(name, 18, (*q.stride()[:3], *kv_pool.stride()[:2], *so)), q.get_device()))
+
+
+def paged_decode_int4(q, kv_pool, block_tables, seq_lens, softmax_scale: Optional[float] = None,
+                      out: Optional[torch.Tensor] = None,
+                      workspace: Optional[DecodeWorkspace] = None) -> torch.Tensor:
+    """q [B, H_kv, N_REP, 128] fp16; kv_pool [num_blocks, H_kv, record] uint8 (see
+    `int4_write`); block_tables [B, max_pages], seq_lens [B] int32 -> [B, H_kv, N_REP, 128] fp16."""
+    if not block_tables.is_contiguous():
+        block_tables = block_tables.contiguous()
+    key = (q.shape, q.stride(), q.dtype, q.get_device(), kv_pool.shape, kv_pool.stride(), kv_pool.dtype,
+           kv_pool.get_device(), block_tables.shape, block_tables.dtype, block_tables.get_device(), seq_lens.shape,
+           seq_lens.stride(), seq_lens.dtype, seq_lens.get_device(),
+           None if out is None else (out.shape, out.stride(), out.dtype, out.get_device()))
+    shape, counts, strides, index = _INT4_LAYOUTS.get(key) or _int4_layout(key, q, kv_pool, block_tables, seq_lens, out)
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    stream = _lib.launch_stream(index)
+    scratch_addresses, *buffers = (workspace or stream_workspace(index, stream)).get(*shape)
     rc = _lib.lib().ls_paged_decode_int4(
-        q.data_ptr(), kv_pool.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(), acc, acc + rows * 512,
-        acc + rows * 516, seg.data_ptr(), out.data_ptr(), b, h, r, i4.groups_of(kv_pool), d, 16,
-        block_tables.shape[1], kv_pool.shape[0], chunks, MIN_CHUNK_PAGES, dense_launch_flags(), sq[0], sq[1], sq[2],
-        sp[0], sp[1], so[0], so[1], so[2], softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(d), stream)
-    _lib.check(rc, "paged_decode_int4")
+        q.data_ptr(), kv_pool.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(), *scratch_addresses,
+        out.data_ptr(), *counts, dense_launch_flags(), *strides,
+        0.08838834764831845 if softmax_scale is None else softmax_scale, stream)
+    if rc:
+        _lib.check(rc, "paged_decode_int4")
     return out
