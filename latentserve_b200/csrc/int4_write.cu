@@ -19,11 +19,14 @@ struct Int4Rows {
     long long sp_b, sp_h;                  // pool strides, bytes
 };
 
-// grid (pages a window of `tokens` positions can touch, H, B), one page of one head per CTA.
-// The last new_lens[b] (or `tokens`) positions of sequence b, [L - m, L), are written from rows
-// 0 .. m - 1. Warp w takes tokens w, w + 4, ..; a token is one warp pass, K in lanes 0-15, V in
-// 16-31. A page that the new rows cover whole is put together in shared memory and stored
-// coalesced; of any other page only the new tokens' own bytes are stored.
+// Token k of warp j's four: 2j, 2j + 1, 2j + 8, 2j + 9, the ones that share words of V codes.
+__device__ __forceinline__ int warp_token(int j, int k) { return 2 * j + (k & 1) + 8 * (k >> 1); }
+
+// grid (pages a window of `tokens` positions can touch, H, B), one page of one head per CTA, four
+// tokens a warp, K in lanes 0-15, V in 16-31. The last new_lens[b] (or `tokens`) positions of
+// sequence b, [L - m, L), are written from rows 0 .. m - 1. A page that the new rows cover whole is
+// put together in shared memory and stored coalesced; of any other page only the new tokens' own
+// bytes are stored.
 template <int G>
 __global__ void __launch_bounds__(kWriteThreads)
 int4_write_kernel(const __half* __restrict__ k, const __half* __restrict__ v, uint8_t* __restrict__ pool,
@@ -39,26 +42,29 @@ int4_write_kernel(const __half* __restrict__ k, const __half* __restrict__ v, ui
     const int page = first / LS_PAGE + blockIdx.x;
     if (page >= r.max_pages || (long long)page * LS_PAGE >= len) return;
     const int blk = r.block_tables[(long long)b * r.max_pages + page];
-    if (blk < 0 || blk >= r.num_blocks) return;          // never write outside the pool
     const int t0 = max(first - page * LS_PAGE, 0), t1 = min(len - page * LS_PAGE, LS_PAGE);
-    const bool whole = t0 == 0 && t1 == LS_PAGE;
-    uint8_t* rec = pool + blk * r.sp_b + h * r.sp_h;
     const __half* src = lane < 16 ? k + b * sk_b + h * sk_h : v + b * sv_b + h * sv_h;
     const long long st = lane < 16 ? sk_t : sv_t;
     uint4 raw[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int t = warp + 4 * i;
+        const int t = warp_token(warp, i);
         raw[i] = make_uint4(0, 0, 0, 0);
         if (t >= t0 && t < t1)
             raw[i] = *reinterpret_cast<const uint4*>(src + (long long)(page * LS_PAGE + t - start) * st + (lane & 15) * 8);
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int t = warp + 4 * i;
-        if (t >= t0 && t < t1) int4_put_token<G>(whole ? image : rec, t, raw[i], lane);
+    if (blk < 0 || blk >= r.num_blocks) return;          // never write outside the pool
+    uint8_t* rec = pool + blk * r.sp_b + h * r.sp_h;
+    if (t0 > 0 || t1 < LS_PAGE) {
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) {
+            const int t = warp_token(warp, i);
+            const uint4 x = i == 0 ? raw[0] : i == 1 ? raw[1] : i == 2 ? raw[2] : raw[3];
+            if (t >= t0 && t < t1) int4_put_token<G>(rec, t, x, lane);
+        }
+        return;
     }
-    if (!whole) return;
+    int4_put_tokens<G>(image, warp, raw, lane);
     __syncthreads();
     for (int i = threadIdx.x; i < int4_record_bytes(G) / 16; i += kWriteThreads)
         reinterpret_cast<uint4*>(rec)[i] = reinterpret_cast<const uint4*>(image)[i];
@@ -86,16 +92,15 @@ int4_read_kernel(const uint8_t* __restrict__ pool, __half* __restrict__ k, __hal
             reinterpret_cast<uint4*>(image)[i] = rec[i];
     }
     __syncthreads();
+    uint4 out[4] = {};
+    if (there) int4_get_tokens<G>(image, warp, lane, out);
     __half* dst = lane < 16 ? k + b * sk_b + h * sk_h : v + b * sv_b + h * sv_h;
     const long long st = lane < 16 ? sk_t : sv_t;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int t = warp + 4 * i;
-        const long long pos = (long long)page * LS_PAGE + t, row = pos - start;
+        const long long pos = (long long)page * LS_PAGE + warp_token(warp, i), row = pos - start;
         if (row < 0 || row >= r.tokens) continue;
-        uint4 out = make_uint4(0, 0, 0, 0);
-        if (there && pos < len) out = int4_get<G>(image, t, lane >> 4, lane & 15);
-        *reinterpret_cast<uint4*>(dst + row * st + (lane & 15) * 8) = out;
+        *reinterpret_cast<uint4*>(dst + row * st + (lane & 15) * 8) = pos < len ? out[i] : make_uint4(0, 0, 0, 0);
     }
 }
 

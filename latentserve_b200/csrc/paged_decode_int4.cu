@@ -61,19 +61,19 @@ __device__ __forceinline__ float half_lo(uint32_t x) { return __low2float(*reint
 __device__ __forceinline__ float half_hi(uint32_t x) { return __high2float(*reinterpret_cast<const __half2*>(&x)); }
 
 // D = A(16x8, fp16, row) * B(8x8, fp16, col).
-__device__ __forceinline__ void mma_1688_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+__device__ __forceinline__ void mma_1688_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0, const float (&z)[4]) {
     asm volatile(
-        "mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};\n"
+        "mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%8,%9,%10};\n"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a0), "r"(a1), "r"(b0), "f"(0.f));
+        : "r"(a0), "r"(a1), "r"(b0), "f"(z[0]), "f"(z[1]), "f"(z[2]), "f"(z[3]));
 }
 // D = A(16x16) * B(16x8): an accumulator that starts here is not cleared first.
 __device__ __forceinline__ void mma_16816_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                              uint32_t b0, uint32_t b1) {
+                                              uint32_t b0, uint32_t b1, const float (&z)[4]) {
     asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};\n"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(z[0]), "f"(z[1]), "f"(z[2]), "f"(z[3]));
 }
 
 // The state of one warp. Lane (g = lane / 4, j = lane % 4).
@@ -86,6 +86,7 @@ struct Int4State {
     float o[9][4];             // O^T tile i < 8: channel 16 i + g of rows 2j, 2j+1 (in 2^-24), channel 16 i + 8 + g
                                // (in 2^-20); tile 8: lanes g < G the sum of w * lo of group g, lanes g = G the sum of w
     float m[2];                // reference of rows 2j, 2j+1 (log2)
+    float zero[4];             // what a new accumulator starts from, in registers of its own
     float f[2];                // softmax scale (log2) over the query's power of two, rows 2j, 2j+1
 
     // This lane's share of the query: row g, channels 32 w + 8 j .. of word w.
@@ -101,6 +102,8 @@ struct Int4State {
 
     __device__ __forceinline__ void begin(const DecodeParams& p, const uint4 (&raw)[4], int lane) {
         m[0] = m[1] = neg_inf();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) asm volatile("mov.f32 %0, 0f00000000;\n" : "=f"(zero[i]));
 #pragma unroll
         for (int i = 0; i < 9; ++i)
 #pragma unroll
@@ -185,12 +188,12 @@ struct Int4State {
             st1[0] = half_lo(low1);
         }
         float base[4], acc[G][4];
-        mma_1688_new(base, low0, low1, qs);
+        mma_1688_new(base, low0, low1, qs, zero);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             const int y = w * G / 4;
             const uint32_t x0 = k0[w], x1 = k1[w], z0 = x0 >> 8, z1 = x1 >> 8;
-            if (w * G % 4 == 0) mma_16816_new(acc[y], x0 & kLow, x1 & kLow, z0 & kLow, z1 & kLow, qb[w][0], qb[w][1]);
+            if (w * G % 4 == 0) mma_16816_new(acc[y], x0 & kLow, x1 & kLow, z0 & kLow, z1 & kLow, qb[w][0], qb[w][1], zero);
             else mma_16816(acc[y], x0 & kLow, x1 & kLow, z0 & kLow, z1 & kLow, qb[w][0], qb[w][1]);
             mma_16816(acc[y], x0 & kHigh, x1 & kHigh, z0 & kHigh, z1 & kHigh, qb[w][2], qb[w][3]);
         }
