@@ -43,6 +43,44 @@ struct Int4Fit {
     __half step, lo;
 };
 
+// The quantiser as its formula reads. Out of line: the usual row does not come here.
+template <int G>
+static __device__ __noinline__ Int4Fit int4_fit_divided(const uint4 raw) {
+    const __half2* h2 = reinterpret_cast<const __half2*>(&raw);
+    Int4Fit fit;
+    float x[8], lo = 65504.f, hi = -65504.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(h2[i]);
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        x[i] = isnan(x[i]) ? 0.f : fminf(fmaxf(x[i], -65504.f), 65504.f);
+        lo = fminf(lo, x[i]);
+        hi = fmaxf(hi, x[i]);
+    }
+#pragma unroll
+    for (int off = 1; off < 16 / G; off <<= 1) {
+        lo = fminf(lo, __shfl_xor_sync(LS_FULL_MASK, lo, off));
+        hi = fmaxf(hi, __shfl_xor_sync(LS_FULL_MASK, hi, off));
+    }
+    fit.step = __float2half_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.f));
+    fit.lo = __float2half_rn(lo);
+    const float t = __half2float(fit.step);
+    fit.codes = 0;
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+        float v = x[0];                                   // (no indexing by i: x stays in registers)
+#pragma unroll
+        for (int k = 1; k < 8; ++k) v = i == k ? x[k] : v;
+        const float u = t > 0.f ? rintf(__fdiv_rn(__fsub_rn(v, lo), t)) : 0.f;
+        fit.codes |= (uint32_t)fminf(fmaxf(u, 0.f), 15.f) << (4 * i);
+    }
+    return fit;
+}
+
 // Eight neighbouring channels a lane, 16 / G lanes a group, a row in 16 lanes; all lanes of the warp
 // take part. lo = min x, step = fp16((max - lo) / 15), code = rne((x - lo) / step), at most 15.
 // NaN counts as 0 and infinities as +-65504: what is stored is always finite, and a step is at
@@ -78,61 +116,32 @@ __device__ __forceinline__ Int4Fit int4_fit(const uint4& raw) {
     asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(s));
     const float magic = 12582912.f;
     const f32x2 lo2 = pack2(-lo, -lo), y2 = pack2(y, y), up = pack2(magic, magic), down = pack2(-magic, -magic), s2 = pack2(-s, -s);
-    uint32_t w = 0;
-    float off_most = 0.f;
+    f32x2 z[4];                                           // codes as floats, two neighbours each
+    float r_first[2], off_most = 0.f;
 #pragma unroll
-    for (int i = 3; i >= 0; --i) {
+    for (int i = 0; i < 4; ++i) {
         const float2 x = __half22float2(h2[i]);
-        const f32x2 d = add2(pack2(x.x, x.y), lo2), r = fma2(d, y2, up), e = fma2(add2(r, down), s2, d);
-        float r0, r1, e0, e1;
-        unpack2(r, r0, r1);
-        unpack2(e, e0, e1);
+        const f32x2 d = add2(pack2(x.x, x.y), lo2), r = fma2(d, y2, up);
+        z[i] = add2(r, down);
+        float e0, e1, skip;
+        unpack2(fma2(z[i], s2, d), e0, e1);
         off_most = fmaxf(off_most, fmaxf(fabsf(e0), fabsf(e1)));
-        w = (w * 16 + __float_as_uint(r1)) * 16 + __float_as_uint(r0);
+        if (i % 2 == 0) unpack2(r, r_first[i / 2], skip);
     }
-    fit.codes = w - 0x3f400000u;                          // 8 nibbles of 0x4b400000, the bits of 1.5 2^23
+    // Four codes make sixteen bits on top of 1.5 2^23, exactly.
+    uint32_t quad[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        float z1, z2, z3, skip;
+        unpack2(z[2 * i], skip, z1);
+        unpack2(z[2 * i + 1], z2, z3);
+        quad[i] = __float_as_uint(fmaf(fmaf(z3, 256.f, z1), 16.f, fmaf(z2, 256.f, r_first[i])));
+    }
+    fit.codes = prmt(quad[0], quad[1], 0x5410);
     const bool plain = range <= 131008.f && range * y < 15.4f && off_most < 0.49999f * s;
     if (__all_sync(LS_FULL_MASK, plain)) return fit;
 
-    float x[8], hi = -65504.f;
-    lo = 65504.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(h2[i]);
-        x[2 * i] = f.x;
-        x[2 * i + 1] = f.y;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        x[i] = isnan(x[i]) ? 0.f : fminf(fmaxf(x[i], -65504.f), 65504.f);
-        lo = fminf(lo, x[i]);
-        hi = fmaxf(hi, x[i]);
-    }
-#pragma unroll
-    for (int off = 1; off < 16 / G; off <<= 1) {
-        lo = fminf(lo, __shfl_xor_sync(LS_FULL_MASK, lo, off));
-        hi = fmaxf(hi, __shfl_xor_sync(LS_FULL_MASK, hi, off));
-    }
-    fit.step = __float2half_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.f));
-    fit.lo = __float2half_rn(lo);
-    const float t = __half2float(fit.step);
-    fit.codes = 0;
-#pragma unroll 1
-    for (int i = 0; i < 8; ++i) {
-        float v = x[0];                                   // (no indexing by i: x stays in registers)
-#pragma unroll
-        for (int k = 1; k < 8; ++k) v = i == k ? x[k] : v;
-        const float u = t > 0.f ? rintf(__fdiv_rn(__fsub_rn(v, lo), t)) : 0.f;
-        fit.codes |= (uint32_t)fminf(fmaxf(u, 0.f), 15.f) << (4 * i);
-    }
-    return fit;
-}
-
-// Nibbles 4 n .. 4 n + 3 of w in the low halves of four bytes.
-__device__ __forceinline__ uint32_t spread_nibbles(uint32_t w, int n) {
-    uint32_t x = n ? w >> 16 : w & 0xffffu;
-    x = (x | (x << 8)) & 0x00ff00ffu;
-    return (x | (x << 4)) & 0x0f0f0f0fu;
+    return int4_fit_divided<G>(raw);
 }
 
 // Bytes k of four words next to one another: out[k] = {w0.k, w1.k, w2.k, w3.k}.
@@ -145,51 +154,98 @@ __device__ __forceinline__ void transpose_bytes(uint32_t w0, uint32_t w1, uint32
     out[3] = prmt(c, d, 0x7632);
 }
 
-// The K codes and the scales of one token, K in lanes 0-15, V in lanes 16-31.
+__device__ __forceinline__ uint32_t half_pair(__half lo, __half hi) {
+    const __half2 h = __halves2half2(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// One token's K codes and scales, lane hl of its sixteen.
 template <int G>
-__device__ __forceinline__ void int4_put_scales(uint8_t* rec, int t, const Int4Fit& fit, int lane) {
-    const int hl = lane & 15, grp = hl / (16 / G);
-    if (lane < 16) *reinterpret_cast<uint32_t*>(rec + 64 * t + 16 * (hl & 3) + 4 * (hl >> 2)) = fit.codes;
-    if (hl % (16 / G) != 0) return;
-    __half* at = reinterpret_cast<__half*>(rec + (lane < 16 ? kI4Scales : int4_v_steps(G)));
-    at += lane < 16 ? 2 * G * t + grp : int4_v_scale_index(G, t, grp);
-    at[0] = fit.step;
-    at[lane < 16 ? G : 16 * G] = fit.lo;
+__device__ __forceinline__ void int4_put_k(uint8_t* rec, int t, const Int4Fit& fit, int hl) {
+    *reinterpret_cast<uint32_t*>(rec + 64 * t + 16 * (hl & 3) + 4 * (hl >> 2)) = fit.codes;
+    if (hl % (16 / G) == 0) {
+        __half* at = reinterpret_cast<__half*>(rec + kI4Scales) + 2 * G * t + hl / (16 / G);
+        at[0] = fit.step;
+        at[G] = fit.lo;
+    }
+}
+
+template <int G>
+__device__ __forceinline__ void int4_put_v_scales(uint8_t* rec, int t, const Int4Fit& fit, int hl) {
+    if (hl % (16 / G) == 0) {
+        __half* at = reinterpret_cast<__half*>(rec + int4_v_steps(G)) + int4_v_scale_index(G, t, hl / (16 / G));
+        at[0] = fit.step;
+        at[16 * G] = fit.lo;
+    }
+}
+
+// A V byte holds channel c of a token in its low nibble and channel c + 8, the neighbouring lane's,
+// in its high one. Of the pair's eight bytes the even lane gets the first four, the odd lane the rest.
+__device__ __forceinline__ uint32_t int4_v_bytes(uint32_t codes, int odd) {
+    const uint32_t other = __shfl_xor_sync(LS_FULL_MASK, codes, 1);
+    // Nibbles a0 a1 a2 a3 b0 b1 b2 b3 (a: the even lane's), then shuffled to a0 b0 a1 b1 a2 b2 a3 b3.
+    uint32_t x = odd ? prmt(other, codes, 0x7632) : prmt(codes, other, 0x5410);
+    uint32_t t = (x ^ (x >> 8)) & 0x0000ff00u;
+    x ^= t ^ (t << 8);
+    t = (x ^ (x >> 4)) & 0x00f000f0u;
+    return x ^ t ^ (t << 4);
+}
+
+// Byte address of row 0 of a lane's V words: tile hl / 2, lanes 4 g + j of the record.
+__device__ __forceinline__ int int4_v_word(int j, int hl) {
+    return kI4V + (hl >> 3) * 512 + (16 * (hl & 1) + j) * 16 + ((hl >> 1) & 3) * 4;
+}
+
+template <int G>
+__device__ __forceinline__ void int4_put_v(uint8_t* rec, int t, const Int4Fit& fit, uint32_t bytes, int hl) {
+    uint8_t* dst = rec + int4_v_word((t & 7) >> 1, hl) + 2 * (t & 1) + (t >> 3);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dst[i * 64] = (uint8_t)(bytes >> (8 * i));
+    int4_put_v_scales<G>(rec, t, fit, hl);
 }
 
 // One token's K row (lanes 0-15) and V row (lanes 16-31), lane hl of a half holding channels
 // 8 hl .. 8 hl + 7, quantised by one warp into the record `rec`: only that token's bytes.
 template <int G>
 __device__ __forceinline__ void int4_put_token(uint8_t* rec, int t, const uint4& raw, int lane) {
-    const int hl = lane & 15;
     const Int4Fit fit = int4_fit<G>(raw);
-    // The V byte of channel c is shared with channel c + 8, the neighbouring lane's.
-    const uint32_t other = __shfl_xor_sync(LS_FULL_MASK, fit.codes, 1);
-    int4_put_scales<G>(rec, t, fit, lane);
-    if (lane < 16) return;
-    const int odd = hl & 1, tile = hl >> 1;
-    const uint32_t bytes = spread_nibbles(odd ? other : fit.codes, odd) | (spread_nibbles(odd ? fit.codes : other, odd) << 4);
-    uint8_t* dst = rec + kI4V + (tile >> 2) * 512 + ((t & 7) >> 1) * 16 + (tile & 3) * 4 + 2 * (t & 1) + (t >> 3);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) dst[(4 * odd + i) * 64] = (uint8_t)(bytes >> (8 * i));
+    const uint32_t bytes = int4_v_bytes(fit.codes, lane & 1);
+    if (lane < 16) int4_put_k<G>(rec, t, fit, lane);
+    else int4_put_v<G>(rec, t, fit, bytes, lane & 15);
 }
 
-// Tokens 2j, 2j + 1, 2j + 8, 2j + 9 of a page, rows as above: the four that share V words.
+// A whole page's rows in a CTA of four warps: warps 0, 1 have K, 2, 3 V, four tokens a half-warp.
+// V tokens 2j, 2j + 1, 2j + 8, 2j + 9 share words of codes, so they are one half-warp's.
+__device__ __forceinline__ int page_token(int warp, int lane, int k) {
+    const int j = 2 * (warp & 1) + (lane >> 4);
+    return warp < 2 ? 4 * j + k : 2 * j + (k & 1) + 8 * (k >> 1);
+}
+
 template <int G>
-__device__ __forceinline__ void int4_put_tokens(uint8_t* rec, int j, const uint4 (&raw)[4], int lane) {
-    const int hl = lane & 15, odd = hl & 1, tile = hl >> 1;
-    uint32_t bytes[4];                                    // of token k: channels of rows 4 odd .. 4 odd + 3 of the tile
+__device__ __forceinline__ void int4_put_page(uint8_t* rec, const uint4 (&raw)[4], int warp, int lane) {
+    const int hl = lane & 15;
+    if (warp < 2) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) int4_put_k<G>(rec, page_token(warp, lane, k), int4_fit<G>(raw[k]), hl);
+        return;
+    }
+    uint32_t bytes[4], words[4];
+    __half steps[4], lows[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         const Int4Fit fit = int4_fit<G>(raw[k]);
-        const uint32_t other = __shfl_xor_sync(LS_FULL_MASK, fit.codes, 1);
-        int4_put_scales<G>(rec, 2 * j + (k & 1) + 8 * (k >> 1), fit, lane);
-        bytes[k] = spread_nibbles(odd ? other : fit.codes, odd) | (spread_nibbles(odd ? fit.codes : other, odd) << 4);
+        bytes[k] = int4_v_bytes(fit.codes, lane & 1);
+        steps[k] = fit.step;
+        lows[k] = fit.lo;
     }
-    if (lane < 16) return;
-    uint32_t words[4];
+    const int j = 2 * (warp & 1) + (lane >> 4);
+    if (hl % (16 / G) == 0) {                                 // [f][e] of the four tokens lie side by side
+        uint8_t* at = rec + int4_v_steps(G) + 8 * G * j + 8 * (hl / (16 / G));
+        *reinterpret_cast<uint2*>(at) = make_uint2(half_pair(steps[0], steps[1]), half_pair(steps[2], steps[3]));
+        *reinterpret_cast<uint2*>(at + 32 * G) = make_uint2(half_pair(lows[0], lows[1]), half_pair(lows[2], lows[3]));
+    }
     transpose_bytes(bytes[0], bytes[2], bytes[1], bytes[3], words);      // byte 2 e + f: tokens 2j, 2j+8, 2j+1, 2j+9
-    uint8_t* dst = rec + kI4V + (tile >> 2) * 512 + (16 * odd + j) * 16 + (tile & 3) * 4;
+    uint8_t* dst = rec + int4_v_word(j, hl);
 #pragma unroll
     for (int i = 0; i < 4; ++i) *reinterpret_cast<uint32_t*>(dst + i * 64) = words[i];
 }
@@ -208,34 +264,40 @@ __device__ __forceinline__ uint4 int4_values(uint32_t b0, uint32_t b1, __half st
     return out;
 }
 
-// The inverse of int4_put_tokens: channels 8 hl .. 8 hl + 7 of the four tokens, K in lanes 0-15, V in 16-31.
+// The inverse of int4_put_page: channels 8 hl .. 8 hl + 7 of page_token(warp, lane, k) into out[k].
 template <int G>
-__device__ __forceinline__ void int4_get_tokens(const uint8_t* rec, int j, int lane, uint4 (&out)[4]) {
-    const int hl = lane & 15, odd = hl & 1, tile = hl >> 1, grp = hl / (16 / G);
-    uint32_t words[4], bytes[4];
+__device__ __forceinline__ void int4_get_page(const uint8_t* rec, int warp, int lane, uint4 (&out)[4]) {
+    const int hl = lane & 15, odd = lane & 1, grp = hl / (16 / G), j = 2 * (warp & 1) + (lane >> 4);
+    uint32_t words[4];
+    __half steps[4], lows[4];
+    if (warp < 2) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int t = 2 * j + (i & 1) + 8 * (i >> 1);
-        words[i] = *reinterpret_cast<const uint32_t*>(
-            lane < 16 ? rec + 64 * t + 16 * (hl & 3) + 4 * (hl >> 2)
-                      : rec + kI4V + (tile >> 2) * 512 + (16 * odd + j) * 16 + (tile & 3) * 4 + i * 64);
+        for (int k = 0; k < 4; ++k) {
+            const int t = page_token(warp, lane, k);
+            const __half* sc = reinterpret_cast<const __half*>(rec + kI4Scales) + 2 * G * t + grp;
+            words[k] = *reinterpret_cast<const uint32_t*>(rec + 64 * t + 16 * (hl & 3) + 4 * (hl >> 2));
+            steps[k] = sc[0];
+            lows[k] = sc[G];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t even = words[k] & 0x0f0f0f0fu, uneven = (words[k] >> 4) & 0x0f0f0f0fu;
+            out[k] = int4_values(prmt(even, uneven, 0x5140), prmt(even, uneven, 0x7362), steps[k], lows[k]);
+        }
+        return;
     }
-    transpose_bytes(words[0], words[1], words[2], words[3], bytes);      // V: byte k = token (0, 8, 1, 9)[k]
+    uint32_t bytes[4];
+    const uint8_t *src = rec + int4_v_word(j, hl), *at = rec + int4_v_steps(G) + 8 * G * j + 8 * grp;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) words[i] = *reinterpret_cast<const uint32_t*>(src + i * 64);
+    *reinterpret_cast<uint2*>(steps) = *reinterpret_cast<const uint2*>(at);
+    *reinterpret_cast<uint2*>(lows) = *reinterpret_cast<const uint2*>(at + 32 * G);
+    transpose_bytes(words[0], words[1], words[2], words[3], bytes);      // bytes[k]: token (0, 8, 1, 9)[k] of the four
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         const uint32_t mine = bytes[(k & 1) * 2 + (k >> 1)], other = __shfl_xor_sync(LS_FULL_MASK, mine, 1);
-        const int t = 2 * j + (k & 1) + 8 * (k >> 1);
-        const __half* sc = reinterpret_cast<const __half*>(rec + (lane < 16 ? kI4Scales : int4_v_steps(G)));
-        sc += lane < 16 ? 2 * G * t + grp : int4_v_scale_index(G, t, grp);
-        uint32_t b0, b1;
-        if (lane < 16) {
-            b0 = spread_nibbles(words[k], 0);
-            b1 = spread_nibbles(words[k], 1);
-        } else {
-            b0 = ((odd ? other : mine) >> (4 * odd)) & 0x0f0f0f0fu;
-            b1 = ((odd ? mine : other) >> (4 * odd)) & 0x0f0f0f0fu;
-        }
-        out[k] = int4_values(b0, b1, sc[0], sc[lane < 16 ? G : 16 * G]);
+        out[k] = int4_values(((odd ? other : mine) >> (4 * odd)) & 0x0f0f0f0fu,
+                             ((odd ? mine : other) >> (4 * odd)) & 0x0f0f0f0fu, steps[k], lows[k]);
     }
 }
 

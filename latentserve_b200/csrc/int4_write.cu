@@ -19,20 +19,16 @@ struct Int4Rows {
     long long sp_b, sp_h;                  // pool strides, bytes
 };
 
-// Token k of warp j's four: 2j, 2j + 1, 2j + 8, 2j + 9, the ones that share words of V codes.
-__device__ __forceinline__ int warp_token(int j, int k) { return 2 * j + (k & 1) + 8 * (k >> 1); }
-
-// grid (pages a window of `tokens` positions can touch, H, B), one page of one head per CTA, four
-// tokens a warp, K in lanes 0-15, V in 16-31. The last new_lens[b] (or `tokens`) positions of
-// sequence b, [L - m, L), are written from rows 0 .. m - 1. A page that the new rows cover whole is
-// put together in shared memory and stored coalesced; of any other page only the new tokens' own
-// bytes are stored.
+// grid (pages a window of `tokens` positions can touch, H, B), one page of one head per CTA: two
+// warps have its K rows, two its V rows (page_token). The last new_lens[b] (or `tokens`) positions of
+// sequence b, [L - m, L), are written from rows 0 .. m - 1. Of a page that the new rows cover whole
+// every store fills 32-byte sectors, straight from registers (through shared memory it was a barrier
+// more and no faster); of any other page only the new tokens' own bytes are stored.
 template <int G>
 __global__ void __launch_bounds__(kWriteThreads)
 int4_write_kernel(const __half* __restrict__ k, const __half* __restrict__ v, uint8_t* __restrict__ pool,
                   const int* __restrict__ new_lens, Int4Rows r, long long sk_b, long long sk_h, long long sk_t,
                   long long sv_b, long long sv_h, long long sv_t) {
-    __shared__ __align__(16) uint8_t image[int4_record_bytes(G)];
     const int h = blockIdx.y, b = blockIdx.z;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int len = r.seq_lens[b];
@@ -43,31 +39,30 @@ int4_write_kernel(const __half* __restrict__ k, const __half* __restrict__ v, ui
     if (page >= r.max_pages || (long long)page * LS_PAGE >= len) return;
     const int blk = r.block_tables[(long long)b * r.max_pages + page];
     const int t0 = max(first - page * LS_PAGE, 0), t1 = min(len - page * LS_PAGE, LS_PAGE);
-    const __half* src = lane < 16 ? k + b * sk_b + h * sk_h : v + b * sv_b + h * sv_h;
-    const long long st = lane < 16 ? sk_t : sv_t;
+    const __half* src = (warp < 2 ? k + b * sk_b + h * sk_h : v + b * sv_b + h * sv_h) + (lane & 15) * 8;
+    const long long st = warp < 2 ? sk_t : sv_t, row0 = (long long)page * LS_PAGE - start;
     uint4 raw[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int t = warp_token(warp, i);
+        const int t = page_token(warp, lane, i);
         raw[i] = make_uint4(0, 0, 0, 0);
-        if (t >= t0 && t < t1)
-            raw[i] = *reinterpret_cast<const uint4*>(src + (long long)(page * LS_PAGE + t - start) * st + (lane & 15) * 8);
+        if (t >= t0 && t < t1) raw[i] = *reinterpret_cast<const uint4*>(src + (row0 + t) * st);
     }
     if (blk < 0 || blk >= r.num_blocks) return;          // never write outside the pool
     uint8_t* rec = pool + blk * r.sp_b + h * r.sp_h;
     if (t0 > 0 || t1 < LS_PAGE) {
 #pragma unroll 1
         for (int i = 0; i < 4; ++i) {
-            const int t = warp_token(warp, i);
-            const uint4 x = i == 0 ? raw[0] : i == 1 ? raw[1] : i == 2 ? raw[2] : raw[3];
-            if (t >= t0 && t < t1) int4_put_token<G>(rec, t, x, lane);
+            const int t = page_token(warp, lane, i);
+            const Int4Fit fit = int4_fit<G>(i == 0 ? raw[0] : i == 1 ? raw[1] : i == 2 ? raw[2] : raw[3]);
+            const uint32_t bytes = int4_v_bytes(fit.codes, lane & 1);
+            if (t < t0 || t >= t1) continue;
+            if (warp < 2) int4_put_k<G>(rec, t, fit, lane & 15);
+            else int4_put_v<G>(rec, t, fit, bytes, lane & 15);
         }
         return;
     }
-    int4_put_tokens<G>(image, warp, raw, lane);
-    __syncthreads();
-    for (int i = threadIdx.x; i < int4_record_bytes(G) / 16; i += kWriteThreads)
-        reinterpret_cast<uint4*>(rec)[i] = reinterpret_cast<const uint4*>(image)[i];
+    int4_put_page<G>(rec, raw, warp, lane);
 }
 
 // grid as above for the window [start[b], start[b] + tokens). Rows at or past the sequence's
@@ -77,7 +72,6 @@ __global__ void __launch_bounds__(kWriteThreads)
 int4_read_kernel(const uint8_t* __restrict__ pool, __half* __restrict__ k, __half* __restrict__ v,
                  const int* __restrict__ starts, Int4Rows r, long long sk_b, long long sk_h, long long sk_t,
                  long long sv_b, long long sv_h, long long sv_t) {
-    __shared__ __align__(16) uint8_t image[int4_record_bytes(G)];
     const int h = blockIdx.y, b = blockIdx.z;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int len = r.seq_lens[b];
@@ -86,21 +80,16 @@ int4_read_kernel(const uint8_t* __restrict__ pool, __half* __restrict__ k, __hal
     int blk = -1;
     if ((long long)page * LS_PAGE < len && page < r.max_pages) blk = r.block_tables[(long long)b * r.max_pages + page];
     const bool there = blk >= 0 && blk < r.num_blocks;
-    if (there) {
-        const uint4* rec = reinterpret_cast<const uint4*>(pool + blk * r.sp_b + h * r.sp_h);
-        for (int i = threadIdx.x; i < int4_record_bytes(G) / 16; i += kWriteThreads)
-            reinterpret_cast<uint4*>(image)[i] = rec[i];
-    }
-    __syncthreads();
     uint4 out[4] = {};
-    if (there) int4_get_tokens<G>(image, warp, lane, out);
-    __half* dst = lane < 16 ? k + b * sk_b + h * sk_h : v + b * sv_b + h * sv_h;
-    const long long st = lane < 16 ? sk_t : sv_t;
+    if (there) int4_get_page<G>(pool + blk * r.sp_b + h * r.sp_h, warp, lane, out);
+    __half* dst = (warp < 2 ? k + b * sk_b + h * sk_h : v + b * sv_b + h * sv_h) + (lane & 15) * 8;
+    const long long st = warp < 2 ? sk_t : sv_t, row0 = (long long)page * LS_PAGE - start;
+    const int end = there ? min(len - page * LS_PAGE, LS_PAGE) : 0;      // tokens of the page that exist
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const long long pos = (long long)page * LS_PAGE + warp_token(warp, i), row = pos - start;
-        if (row < 0 || row >= r.tokens) continue;
-        *reinterpret_cast<uint4*>(dst + row * st + (lane & 15) * 8) = pos < len ? out[i] : make_uint4(0, 0, 0, 0);
+        const int t = page_token(warp, lane, i);
+        if (row0 + t < 0 || row0 + t >= r.tokens) continue;
+        *reinterpret_cast<uint4*>(dst + (row0 + t) * st) = t < end ? out[i] : make_uint4(0, 0, 0, 0);
     }
 }
 
