@@ -86,11 +86,11 @@ static __device__ __noinline__ Int4Fit int4_fit_divided(const uint4 raw) {
 // NaN counts as 0 and infinities as +-65504: what is stored is always finite, and a step is at
 // most 131008 / 15.
 //
-// Computing bounds this, so the usual row goes without a division per channel: code = rne(d y) with
-// y within 2^-23 of 1 / step, by adding and subtracting 1.5 2^23, two channels an instruction. That
-// is the rounded quotient unless it lies within 15 2^-22 of a half; then what the code leaves of
-// d is half a step up to 2^-17 of it. A warp with such a channel, a value that is not finite or a
-// quotient past 15 (subnormal steps) divides.
+// Computing bounds this, so the usual row goes without a division per channel, two channels an
+// instruction: with y the correctly rounded 1 / step, u = d y, the quotient d / step correctly
+// rounded is u + (d - u step) y (Markstein; the fused residual is exact), and adding 1.5 2^23
+// rounds it to an integer, halves to even. A warp with a value that is not finite, or with
+// quotients past 15 (subnormal steps), divides.
 template <int G>
 __device__ __forceinline__ Int4Fit int4_fit(const uint4& raw) {
     const __half2* h2 = reinterpret_cast<const __half2*>(&raw);
@@ -114,18 +114,17 @@ __device__ __forceinline__ Int4Fit int4_fit(const uint4& raw) {
     const float s = __half2float(fit.step);
     float y;
     asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(s));
+    y = s > 0.f ? fmaf(fmaf(-s, y, 1.f), y, y) : 0.f;     // a group of one value has step 0: codes 0
     const float magic = 12582912.f;
     const f32x2 lo2 = pack2(-lo, -lo), y2 = pack2(y, y), up = pack2(magic, magic), down = pack2(-magic, -magic), s2 = pack2(-s, -s);
     f32x2 z[4];                                           // codes as floats, two neighbours each
-    float r_first[2], off_most = 0.f;
+    float r_first[2];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float2 x = __half22float2(h2[i]);
-        const f32x2 d = add2(pack2(x.x, x.y), lo2), r = fma2(d, y2, up);
+        const f32x2 d = add2(pack2(x.x, x.y), lo2), u = mul2(d, y2), r = add2(fma2(fma2(u, s2, d), y2, u), up);
         z[i] = add2(r, down);
-        float e0, e1, skip;
-        unpack2(fma2(z[i], s2, d), e0, e1);
-        off_most = fmaxf(off_most, fmaxf(fabsf(e0), fabsf(e1)));
+        float skip;
         if (i % 2 == 0) unpack2(r, r_first[i / 2], skip);
     }
     // Four codes make sixteen bits on top of 1.5 2^23, exactly.
@@ -138,7 +137,7 @@ __device__ __forceinline__ Int4Fit int4_fit(const uint4& raw) {
         quad[i] = __float_as_uint(fmaf(fmaf(z3, 256.f, z1), 16.f, fmaf(z2, 256.f, r_first[i])));
     }
     fit.codes = prmt(quad[0], quad[1], 0x5410);
-    const bool plain = range <= 131008.f && range * y < 15.4f && off_most < 0.49999f * s;
+    const bool plain = range <= 131008.f && range * y < 15.4f;
     if (__all_sync(LS_FULL_MASK, plain)) return fit;
 
     return int4_fit_divided<G>(raw);

@@ -284,6 +284,26 @@ def test_write_is_bit_exact_and_touches_nothing_else(group, n, lens, new):
     assert np.array_equal(after, expect(before, k, v, lens, new, tables, group))
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_write_rounds_ties_to_even_and_takes_any_range(group):
+    """Rows on coarse lattices, where many quotients are exact halves, rows whose steps are subnormal,
+    rows of one value, and rows with single far values."""
+    rng = np.random.default_rng(group)
+    n = 640
+    k = rng.integers(0, 31, (2, 2, n, 128)) * np.float16(0.5) * 2.0 ** rng.integers(-12, 8, (2, 2, n, 1))
+    v = rng.integers(-20, 20, (2, 2, n, 128)) * 2.0 ** -24 * 2.0 ** rng.integers(0, 6, (2, 2, n, 1))
+    v[:, :, ::7] = 3.0
+    k[:, :, 5::11, 17] = 60000.0
+    k, v = k.astype(np.float16), v.astype(np.float16)
+    step = orc.quantize(k, group)[1].astype(np.float64)
+    left = (k.astype(np.float64) - k.astype(np.float64).reshape(2, 2, n, -1, group).min(-1).repeat(group, -1))
+    assert ((left / step.repeat(group, -1)) % 1 == 0.5).mean() > 0.01            # ties there are
+    dev = device()
+    lens = [n, n + 9]
+    before, after, tables = written(torch.from_numpy(k).to(dev), torch.from_numpy(v).to(dev), lens, None, group)
+    assert np.array_equal(after, expect(before, k, v, lens, None, tables, group))
+
+
 def test_write_from_views_and_special_values():
     """K and V rows as interleaved views of one projection; infinities, NaN, -0, subnormals."""
     dev = device()
