@@ -77,7 +77,12 @@ __device__ __forceinline__ void mma_16816_new(float (&d)[4], uint32_t a0, uint32
 }
 
 // The state of one warp. Lane (g = lane / 4, j = lane % 4).
-template <int G>
+//
+// TWICE (at most four query rows): an MMA has eight columns of rows, so columns 4-7 hold rows 0-3
+// again. The scores come out twice, and where the weights go into the MMAs, columns 0-3 carry
+// their high halves and 4-7 the low ones: one MMA per tile does what takes two otherwise (18
+// MMAs a page instead of 27), and the two sums meet at the end.
+template <int G, bool TWICE>
 struct Int4State {
     static constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
     static constexpr int kRecord = int4_record_bytes(G);
@@ -91,12 +96,12 @@ struct Int4State {
 
     // This lane's share of the query: row g, channels 32 w + 8 j .. of word w.
     static __device__ __forceinline__ void load_query(const DecodeParams& p, int b, int h, int lane, uint4 (&raw)[4]) {
-        const int g = lane >> 2, j = lane & 3;
-        const __half* src = p.q + b * p.sq_b + h * p.sq_h + g * p.sq_m + 8 * j;
+        const int row = TWICE ? (lane >> 2) & 3 : lane >> 2, j = lane & 3;
+        const __half* src = p.q + b * p.sq_b + h * p.sq_h + row * p.sq_m + 8 * j;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             raw[w] = make_uint4(0, 0, 0, 0);
-            if (g < p.n_rep) raw[w] = *reinterpret_cast<const uint4*>(src + 32 * w);
+            if (row < p.n_rep) raw[w] = *reinterpret_cast<const uint4*>(src + 32 * w);
         }
     }
 
@@ -233,8 +238,12 @@ struct Int4State {
             const uint32_t mine = g < G ? 0xffffffffu : 0u, one = g == G ? 0x3c003c00u : 0u;
             lows.x = (lows.x & mine & keep0) | one;
             lows.y = (lows.y & mine & keep1) | one;
-            mma_16816(o[8], lows.x, 0u, lows.y, 0u, w0h, w1h);
-            mma_16816(o[8], lows.x, 0u, lows.y, 0u, w0l, w1l);
+            if (TWICE) {
+                mma_16816(o[8], lows.x, 0u, lows.y, 0u, g < 4 ? w0h : w0l, g < 4 ? w1h : w1l);
+            } else {
+                mma_16816(o[8], lows.x, 0u, lows.y, 0u, w0h, w1h);
+                mma_16816(o[8], lows.x, 0u, lows.y, 0u, w0l, w1l);
+            }
         }
         uint32_t st[2 * G];                          // V steps [group][half]
         if (G == 1) {
@@ -256,6 +265,10 @@ struct Int4State {
             b[2 * y + 1] = hmul2_u32(w1h, t1);
             e[2 * y] = hfma2_u32(w0l, t0, hfma2_u32(w0h, t0, hneg2_u32(b[2 * y])));
             e[2 * y + 1] = hfma2_u32(w1l, t1, hfma2_u32(w1h, t1, hneg2_u32(b[2 * y + 1])));
+            if (TWICE && g >= 4) {
+                b[2 * y] = e[2 * y];
+                b[2 * y + 1] = e[2 * y + 1];
+            }
         }
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -270,8 +283,10 @@ struct Int4State {
                 const uint32_t c0 = x1 & kLow, c1 = x1 & kHigh, c2 = z1 & kLow, c3 = z1 & kHigh;
                 mma_16816(o[tile], a0, a1, a2, a3, b[2 * y0], b[2 * y0 + 1]);
                 mma_16816(o[tile + 1], c0, c1, c2, c3, b[2 * y1], b[2 * y1 + 1]);
-                mma_16816(o[tile], a0, a1, a2, a3, e[2 * y0], e[2 * y0 + 1]);
-                mma_16816(o[tile + 1], c0, c1, c2, c3, e[2 * y1], e[2 * y1 + 1]);
+                if (!TWICE) {
+                    mma_16816(o[tile], a0, a1, a2, a3, e[2 * y0], e[2 * y0 + 1]);
+                    mma_16816(o[tile + 1], c0, c1, c2, c3, e[2 * y1], e[2 * y1 + 1]);
+                }
             }
         }
     }
@@ -331,6 +346,12 @@ struct Int4State {
     __device__ __forceinline__ void finish(float* mo, float* mm, float* ml, int n_rep, int lane) {
         const int g = lane >> 2, j = lane & 3;
         const int r0 = 2 * j, r1 = r0 + 1;
+        if (TWICE) {
+#pragma unroll
+            for (int i = 0; i < 9; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[i][k] += __shfl_xor_sync(LS_FULL_MASK, o[i][k], 2);
+        }
 #pragma unroll
         for (int y = 0; y < G; ++y) {
             const float low0 = __shfl_sync(LS_FULL_MASK, o[8][0], 4 * y + j);
@@ -599,10 +620,10 @@ __device__ __forceinline__ void int4_merge(const DecodeParams& p, int first, int
     __syncthreads();                                          // room and rows are free again
 }
 
-template <int G>
+template <int G, bool TWICE>
 __global__ void __launch_bounds__(kThreads, LS_INT4_CTAS)
 int4_decode_kernel(const __grid_constant__ DecodeParams p) {
-    extern __shared__ __align__(128) unsigned char smem[];
+    extern __shared__ __align__(1024) unsigned char smem[];
     constexpr int PG = kInt4Group, STAGES = kInt4Stages, STAGE_BYTES = PG * int4_record_bytes(G);
     static_assert(kThreads == LS_HEAD_DIM, "a thread per channel where warps' states are summed");
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -668,9 +689,9 @@ int4_decode_kernel(const __grid_constant__ DecodeParams p) {
     }
     if (!has_work) return;
 
-    Int4State<G> st;
+    Int4State<G, TWICE> st;
     uint4 query[4];
-    Int4State<G>::load_query(p, b0, h, lane, query);
+    Int4State<G, TWICE>::load_query(p, b0, h, lane, query);
     int stage = 0, b = b0;
     uint32_t phase = 0;                                   // parity of the stage's mbarrier
     bool refill = false;                                  // whether the slot before this one has been consumed
@@ -702,7 +723,7 @@ int4_decode_kernel(const __grid_constant__ DecodeParams p) {
         }
         const int next = int4_next(cum, p.batch, b, g1);
         const bool more = next < p.batch;
-        if (more) Int4State<G>::load_query(p, next, h, lane, query);
+        if (more) Int4State<G, TWICE>::load_query(p, next, h, lane, query);
         if (guard > 0) __syncthreads();                   // the last sequence's sums have been read
         st.finish(merge_o + warp * p.n_rep * kMergeStride, merge_m + warp * kRP, merge_l + warp * kRP, p.n_rep, lane);
         __syncthreads();
@@ -778,7 +799,7 @@ static int launch_int4(const DecodeParams& p, cudaStream_t stream, bool programm
     const size_t smem = ring + kWarps * kInt4Stages * 16 +
                         sizeof(float) * ((size_t)kWarps * p.n_rep * kMergeStride + 2 * kWarps * kRP) +
                         sizeof(int) * ((size_t)kWarps + 2 + p.batch + 1);
-    auto kern = int4_decode_kernel<G>;
+    auto kern = p.n_rep <= 4 ? int4_decode_kernel<G, true> : int4_decode_kernel<G, false>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return (int)e;
     cudaLaunchConfig_t cfg = {};

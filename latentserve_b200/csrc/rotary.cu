@@ -43,6 +43,40 @@ struct alignas(V * sizeof(T)) Run {
     T v[V];
 };
 
+// Rows are read and written once: past L1, which the tables' rows are better left in.
+template <class T, int V>
+__device__ __forceinline__ Run<T, V> load_run(const T* p) {
+    Run<T, V> r;
+    if constexpr (sizeof(r) == 16) {
+        uint4 x;
+        asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "l"(p));
+        r = *reinterpret_cast<Run<T, V>*>(&x);
+    } else {
+        r.v[0] = *p;
+    }
+    return r;
+}
+
+template <int V>
+__device__ __forceinline__ void load_angles(const float* p, float (&out)[V]) {
+    if constexpr (V % 4 == 0) {
+#pragma unroll
+        for (int k = 0; k < V; k += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(p + k);
+            out[k] = x.x; out[k + 1] = x.y; out[k + 2] = x.z; out[k + 3] = x.w;
+        }
+    } else {
+        out[0] = *p;
+    }
+}
+
+// Two neighbouring channels at once where the type packs them.
+__device__ __forceinline__ void store2(float* d, float a, float b) { d[0] = a; d[1] = b; }
+__device__ __forceinline__ void store2(__half* d, float a, float b) { *reinterpret_cast<__half2*>(d) = __floats2half2_rn(a, b); }
+__device__ __forceinline__ void store2(__nv_bfloat16* d, float a, float b) {
+    *reinterpret_cast<__nv_bfloat162*>(d) = __floats2bfloat162_rn(a, b);
+}
+
 // UNIT = what one thread owns of a head: in the half layout a run of V channels and the run rot / 2
 // further on; interleaved two neighbouring runs; or a run of the channels that are not rotated.
 template <class T, int V, bool INTERLEAVED, int HEADS>
@@ -51,9 +85,10 @@ rotary_kernel(const __grid_constant__ RotaryArgs a) {
     using R = Run<T, V>;
     const unsigned rot_units = a.rot / 2 / V, units = rot_units + (a.dim - a.rot) / V;
     const unsigned idx = blockIdx.x * kRotaryThreads + threadIdx.x;
-    const unsigned unit = idx % units, rest = idx / units;
-    const unsigned split = rest % a.splits, tok = rest / a.splits;
+    const unsigned rest = idx / units, unit = idx - rest * units;
+    const unsigned tok = rest / a.splits, split = rest - tok * a.splits;
     if (tok >= (unsigned)a.tokens) return;
+    const long long pos = a.positions[tok];
     const bool turn = unit < rot_units;
     const int c0 = turn ? (INTERLEAVED ? 2 * V : V) * unit : a.rot + V * (unit - rot_units);
     const int c1 = turn ? (INTERLEAVED ? c0 + V : c0 + a.rot / 2) : c0;
@@ -65,32 +100,43 @@ rotary_kernel(const __grid_constant__ RotaryArgs a) {
         if (head >= total) continue;
         const int w = head >= a.heads[0];
         const T* src = static_cast<const T*>(a.x[w]) + tok * a.sx_t[w] + (head - (w ? a.heads[0] : 0)) * a.sx_h[w];
-        lo[i] = *reinterpret_cast<const R*>(src + c0);
-        if (turn) hi[i] = *reinterpret_cast<const R*>(src + c1);
+        lo[i] = load_run<T, V>(src + c0);
+        if (turn) hi[i] = load_run<T, V>(src + c1);
     }
     if (turn) {
-        const long long pos = a.positions[tok];
         const bool known = pos >= 0 && pos < a.max_pos;
-        const float* cr = a.cos_t + (known ? pos : 0) * a.s_tab + V * unit;
-        const float* sr = a.sin_t + (known ? pos : 0) * a.s_tab + V * unit;
         float c[V], s[V];
+        load_angles<V>(a.cos_t + (known ? pos : 0) * a.s_tab + V * unit, c);
+        load_angles<V>(a.sin_t + (known ? pos : 0) * a.s_tab + V * unit, s);
+        // A position that the tables do not have comes out as NaN.
+        const float mul = known ? a.sign : __int_as_float(0x7fffffff);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            // A position that the tables do not have comes out as NaN.
-            c[k] = known ? cr[k] : __int_as_float(0x7fffffff);
-            s[k] = known ? sr[k] * a.sign : __int_as_float(0x7fffffff);
+            s[k] *= mul;
+            if (!known) c[k] = mul;
         }
 #pragma unroll
         for (int i = 0; i < HEADS; ++i) {
             T* const u = lo[i].v;
             T* const v = hi[i].v;
+            if constexpr (V == 1) {
+                const float p = to_f(u[0]), q = to_f(v[0]);
+                u[0] = from_f<T>(p * c[0] - q * s[0]);
+                v[0] = from_f<T>(q * c[0] + p * s[0]);
+            } else if constexpr (INTERLEAVED) {
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-                T& x = INTERLEAVED ? (2 * k < V ? u[2 * k % V] : v[2 * k % V]) : u[k];
-                T& y = INTERLEAVED ? (2 * k + 1 < V ? u[(2 * k + 1) % V] : v[(2 * k + 1) % V]) : v[k];
-                const float p = to_f(x), q = to_f(y);
-                x = from_f<T>(p * c[k] - q * s[k]);
-                y = from_f<T>(q * c[k] + p * s[k]);
+                for (int k = 0; k < V; ++k) {
+                    T* const at = 2 * k < V ? u + 2 * k : v + (2 * k - V);
+                    const float p = to_f(at[0]), q = to_f(at[1]);
+                    store2(at, p * c[k] - q * s[k], q * c[k] + p * s[k]);
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < V; k += 2) {
+                    const float p0 = to_f(u[k]), p1 = to_f(u[k + 1]), q0 = to_f(v[k]), q1 = to_f(v[k + 1]);
+                    store2(u + k, p0 * c[k] - q0 * s[k], p1 * c[k + 1] - q1 * s[k + 1]);
+                    store2(v + k, q0 * c[k] + p0 * s[k], q1 * c[k + 1] + p1 * s[k + 1]);
+                }
             }
         }
     }
@@ -116,12 +162,16 @@ static int launch_rotary(const RotaryArgs& a, bool interleaved, cudaStream_t str
     return (int)cudaGetLastError();
 }
 
-constexpr int kHeads = 4;
+#ifndef LS_ROTARY_HEADS
+#define LS_ROTARY_HEADS 4
+#endif
+constexpr int kHeads = LS_ROTARY_HEADS;
 
 template <class T>
 static int run_rotary(RotaryArgs& a, bool interleaved, cudaStream_t stream) {
     constexpr int V = 16 / sizeof(T);
-    bool wide = (a.rot / 2) % V == 0 && (a.dim - a.rot) % V == 0;
+    bool wide = (a.rot / 2) % V == 0 && (a.dim - a.rot) % V == 0 && a.s_tab % 4 == 0 &&
+                !((reinterpret_cast<uintptr_t>(a.cos_t) | reinterpret_cast<uintptr_t>(a.sin_t)) & 15);
     for (int w = 0; w < 2; ++w)
         if (a.heads[w])
             wide = wide && !(reinterpret_cast<uintptr_t>(a.x[w]) & 15) && !(reinterpret_cast<uintptr_t>(a.y[w]) & 15) &&
@@ -133,7 +183,8 @@ static int run_rotary(RotaryArgs& a, bool interleaved, cudaStream_t stream) {
     a.splits = many ? (total + kHeads - 1) / kHeads : total;
     if (wide)
         return many ? launch_rotary<T, V, kHeads>(a, interleaved, stream) : launch_rotary<T, V, 1>(a, interleaved, stream);
-    return many ? launch_rotary<T, 1, kHeads>(a, interleaved, stream) : launch_rotary<T, 1, 1>(a, interleaved, stream);
+    a.splits = total;
+    return launch_rotary<T, 1, 1>(a, interleaved, stream);
 }
 
 }  // namespace ls
