@@ -14,6 +14,7 @@ from __future__ import annotations
 import ctypes
 import os
 from ctypes import c_float, c_int, c_int64, c_void_p
+from importlib.util import module_from_spec, spec_from_file_location
 
 import torch
 
@@ -120,34 +121,19 @@ def raw_stream(device_index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(device_index)
 
 
-def launch_stream(device_index: int) -> int:
-    """`raw_stream` for tensors that are known to exist on a CUDA device (no lazy
-    initialisation to look after): the same check, a fraction of its cost."""
-    if torch._C._cuda_getDevice() != device_index:
-        return raw_stream(device_index)                 # says what is wrong
-    return torch._C._cuda_getCurrentRawStream(device_index)
+_BINDING = None
+# Entry points the binding calls, in the order its `bind` takes them.
+_BOUND = ("ls_paged_decode_int4", "ls_int4_write", "ls_int4_read", "ls_copy_pages", "ls_rotary")
 
 
-class Layouts:
-    """What a call works out from its tensors' layouts -- shapes, strides, types, devices -- kept
-    per layout, so that a decode loop's calls check once and launch many times. Nothing about
-    the tensors' contents or addresses is kept; alignment is checked at every call."""
-
-    def __init__(self, limit: int = 4096):
-        self._known: dict = {}
-        self._limit = limit
-
-    def get(self, key):
-        return self._known.get(key)
-
-    def put(self, key, value):
-        if len(self._known) >= self._limit:
-            self._known.clear()
-        self._known[key] = value
-        return value
-
-
-def bound(name: str, first: int, values) -> tuple:
-    """`values` as the C types of entry point `name`'s parameters from number `first` on: a call
-    that is made again and again converts only what changes."""
-    return tuple(kind(v) for kind, v in zip(_PROTOTYPES[name][first:], values, strict=False))
+def binding():
+    """The compiled binding (`csrc/binding.cpp`): launches what needs no explaining, and returns None
+    for everything else, which the Python functions then check step by step."""
+    global _BINDING
+    if _BINDING is None:
+        spec = spec_from_file_location("ls_binding", _build.build_binding())
+        module = module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.bind(*(ctypes.cast(getattr(lib(), name), c_void_p).value for name in _BOUND))
+        _BINDING = module
+    return _BINDING

@@ -17,11 +17,13 @@ import pathlib
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = pathlib.Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 OUT_DIR = HERE / "_C"
 LIB = OUT_DIR / "libls_b200.so"
+BINDING = OUT_DIR / "ls_binding.so"
 SOURCES = ("paged_decode.cu", "kv_write.cu", "page_select.cu", "fused_elementwise.cu",
            "skinny_gemm.cu", "int4_write.cu", "paged_decode_int4.cu",
            "page_copy.cu", "rotary.cu")
@@ -72,6 +74,34 @@ def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = Fals
     return pathlib.Path(out)
 
 
+def build_binding(force: bool = False, verbose: bool = False) -> pathlib.Path:
+    """The CPython module over the library's C ABI (csrc/binding.cpp), against the installed
+    torch's headers: host code only, no GPU and no nvcc needed."""
+    source = CSRC / "binding.cpp"
+    deps = [source, *HERE.parent.glob("include/*.h")]
+    if not force and BINDING.exists() and all(p.stat().st_mtime <= BINDING.stat().st_mtime for p in deps):
+        return BINDING
+    import torch
+
+    cxx = os.environ.get("CXX") or shutil.which("g++") or shutil.which("c++")
+    if not cxx:
+        raise RuntimeError("no C++ compiler found for the binding")
+    root = pathlib.Path(torch.__file__).resolve().parent
+    OUT_DIR.mkdir(exist_ok=True)
+    cmd = [cxx, "-shared", "-fPIC", "-O2", "-std=c++17", f"-I{root / 'include'}",
+           f"-I{root / 'include/torch/csrc/api/include'}", f"-I{pathlib.Path(nvcc_path()).parent.parent / 'include'}",
+           f"-I{sysconfig.get_paths()['include']}", str(source), "-o", str(BINDING), f"-L{root / 'lib'}", "-lc10",
+           "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    if verbose:
+        print(" ".join(cmd), file=sys.stderr)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"{cxx} failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+    return BINDING
+
+
 if __name__ == "__main__":
     path = build(force="--force" in sys.argv, verbose=True, ptxas_verbose="--ptxas" in sys.argv)
     print(path)
+    if not os.environ.get("LS_LIB_OUT"):
+        print(build_binding(force="--force" in sys.argv, verbose=True))

@@ -68,9 +68,6 @@ def _vector(t: torch.Tensor, batch: int, device, what: str) -> torch.Tensor:
     return t
 
 
-_WRITES, _READS = _lib.Layouts(), _lib.Layouts()
-
-
 def _strides(t: torch.Tensor) -> list[int]:
     """Batch, head and token stride; 0 for an axis of one, whose stride says nothing."""
     return [st if n > 1 else 0 for n, st in zip(t.shape[:3], t.stride()[:3])]
@@ -102,30 +99,21 @@ def write(k: torch.Tensor, v: torch.Tensor, kv_pool: torch.Tensor, block_tables:
     they are. A page that two sequences of the batch write at the same position holds either.
 
     NaN is stored as 0 and an infinity as the largest fp16 of its sign."""
-    if not block_tables.is_contiguous():
-        block_tables = block_tables.contiguous()
-    key = (k.shape, k.stride(), k.dtype, k.get_device(), v.shape, v.stride(), v.dtype, v.get_device(), kv_pool.shape,
-           kv_pool.stride(), kv_pool.dtype, kv_pool.get_device(), block_tables.shape, block_tables.dtype,
-           block_tables.get_device(), seq_lens.shape, seq_lens.stride(), seq_lens.dtype, seq_lens.get_device(),
-           None if new_lens is None else (new_lens.shape, new_lens.stride(), new_lens.dtype, new_lens.get_device()))
-    known = _WRITES.get(key)
-    if known is None:
-        _check_rows(k, v, kv_pool)
-        b, h, n, d = k.shape
-        check_tables(block_tables, seq_lens, b, k.device)
-        if new_lens is not None:
-            _vector(new_lens, b, k.device, "new_lens")
-        args = (b, h, n, groups_of(kv_pool), d, 16, block_tables.shape[1], kv_pool.shape[0], *_strides(k), *_strides(v),
-                *kv_pool.stride()[:2])
-        known = _WRITES.put(key, (_lib.bound("ls_int4_write", 6, args), k.get_device(), b * n > 0))
-    args, index, some = known
-    if not some:
+    if _lib.binding().write(k, v, kv_pool, block_tables, seq_lens, new_lens) is not None:
         return
-    rc = _lib.lib().ls_int4_write(k.data_ptr(), v.data_ptr(), kv_pool.data_ptr(), block_tables.data_ptr(),
-                                  seq_lens.data_ptr(), 0 if new_lens is None else new_lens.data_ptr(), *args,
-                                  _lib.launch_stream(index))
-    if rc:
-        _lib.check(rc, "int4 write")
+    _check_rows(k, v, kv_pool)
+    b, h, n, d = k.shape
+    block_tables = check_tables(block_tables, seq_lens, b, k.device)
+    if new_lens is not None:
+        _vector(new_lens, b, k.device, "new_lens")
+    if b == 0 or n == 0:
+        return
+    sp = kv_pool.stride()
+    rc = _lib.lib().ls_int4_write(
+        k.data_ptr(), v.data_ptr(), kv_pool.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(),
+        _lib.ptr(new_lens), b, h, n, groups_of(kv_pool), d, 16, block_tables.shape[1], kv_pool.shape[0],
+        *_strides(k), *_strides(v), sp[0], sp[1], _lib.raw_stream(k.device.index))
+    _lib.check(rc, "int4 write")
 
 
 def read(kv_pool: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor, length: int,
@@ -134,38 +122,29 @@ def read(kv_pool: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tens
     start[b] .. start[b] + length - 1 (`start` [B] int32, not negative; zeros if not given).
     Rows at or past seq_lens[b], or of a block outside the pool, are zeros. For what attends a
     cached prefix densely: a prompt's next chunk, a check."""
-    if not block_tables.is_contiguous():
-        block_tables = block_tables.contiguous()
-    key = (length, kv_pool.shape, kv_pool.stride(), kv_pool.dtype, kv_pool.get_device(), block_tables.shape,
-           block_tables.dtype, block_tables.get_device(), seq_lens.shape, seq_lens.stride(), seq_lens.dtype,
-           seq_lens.get_device(),
-           None if start is None else (start.shape, start.stride(), start.dtype, start.get_device()))
-    known = _READS.get(key)
-    if known is None:
-        if not kv_pool.is_cuda:
-            raise RuntimeError("latentserve_b200 has no CPU path: tensors must be on a CUDA device")
-        if length < 0:
-            raise ValueError(f"cannot read {length} positions")
-        if not pool_ok(kv_pool):
-            raise ValueError("kv_pool must be uint8 [num_blocks, H, record_bytes(group)] with 16-byte aligned rows")
-        b, h = seq_lens.shape[0] if seq_lens.dim() else 0, kv_pool.shape[1]
-        check_tables(block_tables, seq_lens, b, kv_pool.device)
-        if start is not None:
-            _vector(start, b, kv_pool.device, "start")
-        rows = (h * length * 128, length * 128, 128)
-        args = (b, h, length, groups_of(kv_pool), 128, 16, block_tables.shape[1], kv_pool.shape[0], *rows, *rows,
-                *kv_pool.stride()[:2])
-        known = _READS.put(key, ((2, b, h, length, 128), kv_pool.device, kv_pool.get_device(),
-                                 _lib.bound("ls_int4_read", 6, args)))
-    shape, device, index, args = known
-    both = torch.empty(shape, dtype=torch.float16, device=device)
-    k, v = both.unbind(0)
-    if shape[1] and shape[2] and length:
-        rc = _lib.lib().ls_int4_read(kv_pool.data_ptr(), k.data_ptr(), v.data_ptr(), block_tables.data_ptr(),
-                                     seq_lens.data_ptr(), 0 if start is None else start.data_ptr(), *args,
-                                     _lib.launch_stream(index))
-        if rc:
-            _lib.check(rc, "int4 read")
+    got = _lib.binding().read(kv_pool, block_tables, seq_lens, length, start)
+    if got is not None:
+        return got
+    if not kv_pool.is_cuda:
+        raise RuntimeError("latentserve_b200 has no CPU path: tensors must be on a CUDA device")
+    if length < 0:
+        raise ValueError(f"cannot read {length} positions")
+    if not pool_ok(kv_pool):
+        raise ValueError("kv_pool must be uint8 [num_blocks, H, record_bytes(group)] with 16-byte aligned rows")
+    b, h, dev = seq_lens.shape[0] if seq_lens.dim() else 0, kv_pool.shape[1], kv_pool.device
+    block_tables = check_tables(block_tables, seq_lens, b, dev)
+    if start is not None:
+        _vector(start, b, dev, "start")
+    k = torch.empty(b, h, length, 128, dtype=torch.float16, device=dev)
+    v = torch.empty_like(k)
+    if k.numel() == 0:
+        return k, v
+    rows, sp = (h * length * 128, length * 128, 128), kv_pool.stride()
+    rc = _lib.lib().ls_int4_read(
+        kv_pool.data_ptr(), k.data_ptr(), v.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(),
+        _lib.ptr(start), b, h, length, groups_of(kv_pool), 128, 16, block_tables.shape[1], kv_pool.shape[0],
+        *rows, *rows, sp[0], sp[1], _lib.raw_stream(dev.index))
+    _lib.check(rc, "int4 read")
     return k, v
 
 

@@ -67,9 +67,8 @@ class PagePools:
         if not s or not self.pools:
             return
         rc = _lib.lib().ls_copy_pages(self.table, len(self.pools), s.buffer_info()[0], d.buffer_info()[0], len(s),
-                                      self.blocks, _lib.launch_stream(self.index))
-        if rc:
-            _lib.check(rc, "copy_pages")
+                                      self.blocks, _lib.raw_stream(self.index))
+        _lib.check(rc, "copy_pages")
 
 
 def copy_pages(pools: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[int], block_dim: int = 0) -> None:
@@ -78,4 +77,5 @@ def copy_pages(pools: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[
     host sequences of page ids: they are read before the call returns, and a captured call
     replays with the same ids. A source may serve several destinations; a destination given
     twice, or that is a source as well, is refused."""
-    PagePools(pools, block_dim).copy(src, dst)
+    if _lib.binding().copy_pages(pools, src, dst, block_dim) is None:
+        PagePools(pools, block_dim).copy(src, dst)

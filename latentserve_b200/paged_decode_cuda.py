@@ -307,21 +307,23 @@ def plan_decode(q, k_pool, v_pool, block_tables, seq_lens, num_splits=None, soft
 
 class DecodeWorkspace:
     """The scratch of 4-bit decode launches that follow one another on the GPU: per (batch, KV
-    heads, partial states) the partial states and an int32 buffer whose arrival counters every
+    heads) the partial states and an int32 buffer whose arrival counters every
     launch leaves at zero. Launches that may overlap -- on two streams, in two captured graphs --
     need one each. A cache owns one for its own decode steps; calls without one get one per stream."""
 
     def __init__(self):
         self._held: dict = {}
 
-    def get(self, batch: int, kv_heads: int, rows: int, device) -> tuple:
-        """(addresses of the partial states and the bookkeeping, the two buffers)"""
-        key = (batch, kv_heads, rows, device)
+    def get(self, batch: int, kv_heads: int, device_index: int) -> tuple:
+        """(addresses of the partial states and the bookkeeping, most chunks, the two buffers)"""
+        key = (batch, kv_heads, device_index)
         held = self._held.get(key)
         if held is None:
-            part = torch.empty(rows * 130, dtype=torch.float32, device=device)
+            device = torch.device("cuda", device_index)
+            chunks = choose_chunks(device, kv_heads, None, batch, INT4_CTAS_PER_SM)
+            part = torch.empty((batch + chunks) * kv_heads * ROWS_PER_PARTIAL * 130, dtype=torch.float32, device=device)
             seg = torch.zeros(seg_len(batch, kv_heads), dtype=torch.int32, device=device)
-            held = (part.data_ptr(), seg.data_ptr()), part, seg
+            held = part.data_ptr(), seg.data_ptr(), chunks, part, seg
             # Made while a graph is being captured, the buffers belong to that graph, which
             # zeroes the counters at every replay: not for anyone else.
             if not torch.cuda.is_current_stream_capturing():
@@ -330,8 +332,8 @@ class DecodeWorkspace:
 
     def error_flag(self, device, batch: int, kv_heads: int) -> int:
         """As `error_flag` above, for launches that used this workspace."""
-        return max((int(seg[2 * batch].item()) for (b, h, _, dev), (_, _, seg) in self._held.items()
-                    if (b, h, dev) == (batch, kv_heads, torch.device(device))), default=0)
+        held = self._held.get((batch, kv_heads, torch.device(device).index))
+        return 0 if held is None else int(held[-1][2 * batch].item())
 
 
 _STREAM_WORKSPACES: dict = {}
@@ -356,11 +358,20 @@ def int4_eligible(q: torch.Tensor, kv_pool: torch.Tensor) -> bool:
             and _aligned(q, 16) and i4.pool_ok(kv_pool) and kv_pool.shape[1] == q.shape[1])
 
 
-_INT4_LAYOUTS = _lib.Layouts()
-
-
-def _int4_layout(key, q, kv_pool, block_tables, seq_lens, out):
-    """The arguments of a 4-bit decode launch that its tensors' layouts decide, after checking them."""
+def paged_decode_int4(q, kv_pool, block_tables, seq_lens, softmax_scale: Optional[float] = None,
+                      out: Optional[torch.Tensor] = None,
+                      workspace: Optional[DecodeWorkspace] = None) -> torch.Tensor:
+    """q [B, H_kv, N_REP, 128] fp16; kv_pool [num_blocks, H_kv, record] uint8 (see
+    `int4_write`); block_tables [B, max_pages], seq_lens [B] int32 -> [B, H_kv, N_REP, 128] fp16."""
+    scale = _SCALE if softmax_scale is None else softmax_scale
+    if q.is_cuda and q.dim() == 4 and 1 <= q.shape[0] <= MAX_BATCH and q.shape[1] >= 1:
+        index = q.get_device()
+        work = workspace or stream_workspace(index, torch._C._cuda_getCurrentRawStream(index))
+        part, seg, chunks, *buffers = work.get(q.shape[0], q.shape[1], index)
+        got = _lib.binding().decode(q, kv_pool, block_tables, seq_lens, out, scale, part, seg, chunks, INT4_MIN_CHUNK,
+                                    dense_launch_flags())
+        if got is not None:
+            return got
     if not q.is_cuda:
         raise RuntimeError("latentserve_b200 has no CPU path: tensors must be on a CUDA device")
     if not int4_eligible(q, kv_pool):
@@ -368,42 +379,23 @@ def _int4_layout(key, q, kv_pool, block_tables, seq_lens, out):
             "layout not supported by the sm_100a kernels: need fp16 q with head_dim 128, <= 8 query rows per KV "
             "head, 1 to 1024 sequences and a uint8 pool of 4-bit page records with 16-byte aligned rows")
     b, h, r, d = q.shape
-    i4.check_tables(block_tables, seq_lens, b, q.device)
+    block_tables = i4.check_tables(block_tables, seq_lens, b, q.device)
     if kv_pool.device != q.device:
         raise ValueError("q and the pool must be on one device")
-    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device
-                            or out.stride(-1) != 1 or any(st % 4 for st in out.stride()[:-1])):
-        raise ValueError("out must be an fp16 [B, H_kv, N_REP, 128] tensor on q's device with 8-byte aligned "
-                         "rows of unit-stride channels")
-    chunks = choose_chunks(q.device, h, None, b, INT4_CTAS_PER_SM)
-    rows = (b + chunks) * h * ROWS_PER_PARTIAL
-    counts = (b, h, r, i4.groups_of(kv_pool), d, 16, block_tables.shape[1], kv_pool.shape[0], chunks, INT4_MIN_CHUNK)
-    so = out.stride()[:3] if out is not None else (h * r * d, r * d, d)
-    name = "ls_paged_decode_int4"
-    return _INT4_LAYOUTS.put(key, ((b, h, rows, q.device), _lib.bound(name, 7, counts),
-                                   _lib.bound(name, 18, (*q.stride()[:3], *kv_pool.stride()[:2], *so)), q.get_device()))
-
-
-def paged_decode_int4(q, kv_pool, block_tables, seq_lens, softmax_scale: Optional[float] = None,
-                      out: Optional[torch.Tensor] = None,
-                      workspace: Optional[DecodeWorkspace] = None) -> torch.Tensor:
-    """q [B, H_kv, N_REP, 128] fp16; kv_pool [num_blocks, H_kv, record] uint8 (see
-    `int4_write`); block_tables [B, max_pages], seq_lens [B] int32 -> [B, H_kv, N_REP, 128] fp16."""
-    if not block_tables.is_contiguous():
-        block_tables = block_tables.contiguous()
-    key = (q.shape, q.stride(), q.dtype, q.get_device(), kv_pool.shape, kv_pool.stride(), kv_pool.dtype,
-           kv_pool.get_device(), block_tables.shape, block_tables.dtype, block_tables.get_device(), seq_lens.shape,
-           seq_lens.stride(), seq_lens.dtype, seq_lens.get_device(),
-           None if out is None else (out.shape, out.stride(), out.dtype, out.get_device()))
-    shape, counts, strides, index = _INT4_LAYOUTS.get(key) or _int4_layout(key, q, kv_pool, block_tables, seq_lens, out)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    stream = _lib.launch_stream(index)
-    scratch_addresses, *buffers = (workspace or stream_workspace(index, stream)).get(*shape)
+    elif (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(-1) != 1
+          or any(st % 4 for st in out.stride()[:-1])):
+        raise ValueError("out must be an fp16 [B, H_kv, N_REP, 128] tensor on q's device with 8-byte aligned "
+                         "rows of unit-stride channels")
+    sq, sp, so = q.stride(), kv_pool.stride(), out.stride()
     rc = _lib.lib().ls_paged_decode_int4(
-        q.data_ptr(), kv_pool.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(), *scratch_addresses,
-        out.data_ptr(), *counts, dense_launch_flags(), *strides,
-        0.08838834764831845 if softmax_scale is None else softmax_scale, stream)
-    if rc:
-        _lib.check(rc, "paged_decode_int4")
+        q.data_ptr(), kv_pool.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(), part, seg, out.data_ptr(), b, h, r,
+        i4.groups_of(kv_pool), d, 16, block_tables.shape[1], kv_pool.shape[0], chunks, INT4_MIN_CHUNK,
+        dense_launch_flags(), sq[0], sq[1], sq[2], sp[0], sp[1], so[0], so[1], so[2], scale,
+        _lib.raw_stream(q.device.index))
+    _lib.check(rc, "paged_decode_int4")
     return out
+
+
+_SCALE = 1.0 / math.sqrt(128)

@@ -97,37 +97,9 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch
     cos, sin fp32 [max_pos, r / 2] say how much of a head turns: its first r channels, in pairs
     (i, i + r / 2), or (2 i, 2 i + 1) with `interleaved`; the rest is copied. `inverse` turns the
     other way, which is also the gradient. A position outside the tables comes out as NaN."""
-    key = (q.shape, q.stride(), q.dtype, q.get_device(), k.shape, k.stride(), k.dtype, k.get_device(), cos.shape,
-           cos.stride(), cos.dtype, cos.get_device(), sin.shape, sin.stride(), sin.dtype, sin.get_device(), positions.shape,
-           positions.stride(), positions.dtype, positions.get_device(), interleaved, inverse,
-           None if q_out is None else (q_out.shape, q_out.stride(), q_out.dtype, q_out.get_device()),
-           None if k_out is None else (k_out.shape, k_out.stride(), k_out.dtype, k_out.get_device()))
-    known = _LAYOUTS.get(key)
-    if known is None:
-        known = _LAYOUTS.put(key, _layout(q, k, cos, sin, positions, interleaved, inverse, q_out, k_out))
-    index, args, some = known
-    if q_out is None:
-        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    if k_out is None:
-        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
-    if not some:
-        return q_out, k_out
-    qp, kp, qo, ko = q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr()
-    if (qp == qo and qp and q.numel() and _strides(q) != _strides(q_out)) or (
-            kp == ko and kp and k.numel() and _strides(k) != _strides(k_out)):
-        raise ValueError("rotating in place needs the output's strides to be the input's")
-    rc = _lib.lib().ls_rotary(qp, kp, qo, ko, cos.data_ptr(), sin.data_ptr(), positions.data_ptr(), *args,
-                              _lib.launch_stream(index))
-    if rc:
-        _lib.check(rc, "apply_rotary")
-    return q_out, k_out
-
-
-_LAYOUTS = _lib.Layouts()
-
-
-def _layout(q, k, cos, sin, positions, interleaved, inverse, q_out, k_out):
-    """Checks a call's layouts and works out the arguments that they decide."""
+    got = _lib.binding().rotary(q, k, cos, sin, positions, interleaved, inverse, q_out, k_out)
+    if got is not None:
+        return got
     if not q.is_cuda:
         raise RuntimeError("latentserve_b200 has no CPU path: tensors must be on a CUDA device")
     if q.dtype not in _DTYPES:
@@ -148,17 +120,25 @@ def _layout(q, k, cos, sin, positions, interleaved, inverse, q_out, k_out):
     if positions.dtype != torch.int64 or positions.shape != (tokens,) or positions.device != q.device or (
             tokens > 1 and positions.stride(0) != 1):
         raise ValueError("positions must be a contiguous int64 vector with one entry per token")
-    strides = [*_strides(q), *_strides(k)]
+    outs = []
     for x, out, what in ((q, q_out, "q_out"), (k, k_out, "k_out")):
         if out is None:
-            strides += [x.shape[1] * dim, dim]
-            continue
+            out = torch.empty_like(x, memory_format=torch.contiguous_format)
         _check(out, tokens, dim, q, what)
         if out.shape != x.shape:
             raise ValueError(f"{what} must have its input's shape")
         if any(size > 1 and stride == 0 for size, stride in zip(out.shape, out.stride())):
             raise ValueError(f"{what} must not be broadcast")
-        strides += _strides(out)
-    args = (tokens, q.shape[1], k.shape[1], dim, rot, _DTYPES[q.dtype], int(interleaved), int(inverse), cos.shape[0],
-            cos.stride(0) if cos.shape[0] > 1 else cos.shape[1], *strides)
-    return q.get_device(), _lib.bound("ls_rotary", 7, args), tokens > 0 and q.shape[1] + k.shape[1] > 0
+        if x.numel() and out.data_ptr() == x.data_ptr() and _strides(out) != _strides(x):
+            raise ValueError(f"{what} in place needs its input's strides")
+        outs.append(out)
+    q_out, k_out = outs
+    if tokens == 0 or q.shape[1] + k.shape[1] == 0:
+        return q_out, k_out
+    rc = _lib.lib().ls_rotary(
+        q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+        positions.data_ptr(), tokens, q.shape[1], k.shape[1], dim, rot, _DTYPES[q.dtype], int(interleaved), int(inverse),
+        cos.shape[0], cos.stride(0) if cos.shape[0] > 1 else cos.shape[1], *_strides(q), *_strides(k), *_strides(q_out),
+        *_strides(k_out), _lib.raw_stream(q.device.index))
+    _lib.check(rc, "apply_rotary")
+    return q_out, k_out

@@ -178,3 +178,24 @@ def test_rotary_tables_keep_far_positions():
     cos, sin = rotary.rotary_tables(4, 1_000_001, 1e4, device="cpu")
     far = 1_000_000
     assert abs(float(cos[far, 0]) - math.cos(far)) < 2.0 ** -23 and abs(float(sin[far, 0]) - math.sin(far)) < 2.0 ** -23
+
+
+def test_binding_declines_what_it_does_not_know():
+    """Anything but CUDA tensors of the usual layout: None, no exception, nothing touched."""
+    fast = _lib.binding()
+    x = torch.zeros(2, 2, 3, 128, dtype=torch.float16)
+    pool, tables = torch.zeros(4, 2, 2560, dtype=torch.uint8), torch.zeros(2, 2, dtype=torch.int32)
+    lens = torch.ones(2, dtype=torch.int32)
+    assert fast.decode(x, pool, tables, lens, None, 0.1, 0, 0, 1, 1, 0) is None
+    assert fast.decode(x, pool) is None and fast.decode(1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11) is None
+    assert fast.write(x, x, pool, tables, lens, None) is None and fast.write(None, x, pool, tables, lens, lens) is None
+    assert fast.write(x, x, pool, tables, None, None) is None
+    assert fast.read(pool, tables, lens, 4, None) is None and fast.read(pool, tables, lens, "4", None) is None
+    assert fast.copy_pages([pool], [0], [1], 0) is None and fast.copy_pages([], [], [], 0) is None
+    assert fast.copy_pages((pool,), [0], [1], 0) is None and fast.copy_pages([pool], [0], [1], 7) is None
+    y = torch.zeros(3, 2, 64)
+    assert fast.rotary(y, y, torch.zeros(4, 32), torch.zeros(4, 32), torch.arange(3), False, False, None, None) is None
+    with pytest.raises(TypeError):
+        fast.bind(1)
+    with pytest.raises(ValueError):
+        fast.bind(0, 0, 0, 0, 0)
