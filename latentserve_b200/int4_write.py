@@ -96,7 +96,8 @@ def write(k: torch.Tensor, v: torch.Tensor, kv_pool: torch.Tensor, block_tables:
     0 .. m-1 of sequence b go to positions seq_lens[b] - m .. seq_lens[b] - 1, m = n or, with
     `new_lens` [B] int32, min(new_lens[b], n); rows past m are not read. Positions below zero,
     past the table or in a block outside the pool are dropped. Bytes of other tokens stay as
-    they are. A page that two sequences of the batch write at the same position holds either.
+    they are. Sequences of one call must not write the same token of the same block (pages that are
+    shared are full): which of the rows' bytes it then holds is not defined.
 
     NaN is stored as 0 and an infinity as the largest fp16 of its sign."""
     if _lib.binding().write(k, v, kv_pool, block_tables, seq_lens, new_lens) is not None:

@@ -163,6 +163,68 @@ def test_attention_skips_blocks_outside_the_pool():
     assert work.error_flag(device(), 2, 2) == 1
 
 
+def test_attention_nothing_to_attend():
+    """All lengths zero or negative, and sequences none of whose blocks lie in the pool: zeros."""
+    q = np.random.default_rng(1).standard_normal((3, 2, 6, 128)).astype(np.float16)
+    pool, tables = make_pool([64, 64, 64], 2, 32, seed=6)
+    for lens in ([0, 0, 0], [-5, 0, -1]):
+        assert (attend(q, pool, tables, lens) == 0).all()
+    tables[1:] = 10 ** 6
+    got = attend(q, pool, tables, [64, 64, 7])
+    assert (got[1:] == 0).all()
+    check(got[:1], q[:1], pool, tables[:1], [64])
+
+
+@pytest.mark.parametrize("rep", [1, 4, 8])
+def test_attention_one_long_sequence(rep):
+    """More partial states than fit the merge's shared memory at once."""
+    lens = [40001]
+    q = np.random.default_rng(rep).standard_normal((1, 1, rep, 128)).astype(np.float16)
+    pool, tables = make_pool(lens, 1, 128, seed=rep)
+    check(attend(q, pool, tables, lens), q, pool, tables, lens)
+
+
+@pytest.mark.parametrize("batch", [65, 300, 1024])
+def test_attention_many_sequences(batch):
+    """More sequences than chunks, than threads; empty ones among them; a workspace used at
+    several batch sizes in turn."""
+    rng = np.random.default_rng(batch)
+    lens = rng.integers(0, 90, batch).tolist()
+    q = rng.standard_normal((batch, 2, 3, 128)).astype(np.float16)
+    pool, tables = make_pool(lens, 2, 64, seed=batch)
+    work = pdc.DecodeWorkspace()
+    for n in (batch, 7, batch, batch // 2):
+        check(attend(q[:n], pool, tables[:n], lens[:n], workspace=work), q[:n], pool, tables[:n], lens[:n])
+    assert work.error_flag(device(), batch, 2) == 0
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1, 1e-6, 0.5])
+def test_attention_scales(scale):
+    lens = [200, 33]
+    q = np.random.default_rng(2).standard_normal((2, 2, 5, 128)).astype(np.float16)
+    pool, tables = make_pool(lens, 2, 32, seed=8)
+    got = attend(q, pool, tables, lens, softmax_scale=scale).float().cpu().numpy()
+    want, _ = orc.attention(q, pool, tables, np.asarray(lens), scale)
+    _, bound = orc.attention(q, pool, tables, np.asarray(lens), abs(scale))
+    wide, _ = orc.attention(-q if scale < 0 else q, pool, tables, np.asarray(lens), abs(scale))
+    assert np.allclose(want, wide, rtol=1e-12, atol=1e-12)
+    # The bound's terms are those of |scale|; its first one is the output's own.
+    assert (np.abs(got - want) <= bound + 2.0 ** -11 * np.abs(want)).all()
+
+
+def test_a_query_that_is_not_finite_spoils_its_own_row_only():
+    lens = [100]
+    q = np.random.default_rng(3).standard_normal((1, 2, 6, 128)).astype(np.float16)
+    pool, tables = make_pool(lens, 2, 32, seed=9)
+    want = attend(q, pool, tables, lens)
+    q[0, 1, 2, 5] = np.nan
+    got = attend(q, pool, tables, lens)
+    assert got[0, 1, 2].isnan().all()
+    keep = torch.ones(2, 6, dtype=torch.bool)
+    keep[1, 2] = False
+    assert torch.equal(got[0][keep.to(got.device)], want[0][keep.to(got.device)])
+
+
 def test_attention_refusals():
     dev = device()
     q = torch.zeros(2, 2, 6, 128, dtype=torch.float16, device=dev)
@@ -350,6 +412,29 @@ def test_read_gives_the_rounded_values(group):
                         one = [x[p % 16: p % 16 + 1] for x in part]
                         want[side, b, h, p - first] = orc.dequantize(*one)[0].astype(np.float32).astype(np.float16)
         assert np.array_equal(k.cpu().numpy(), want[0]) and np.array_equal(v.cpu().numpy(), want[1])
+
+
+def test_blocks_past_four_gigabytes():
+    """A pool of 5.4 GB: write, copy, read and attend pages at its far end."""
+    from latentserve_b200 import page_copy
+
+    dev = device()
+    nb = 1_050_000
+    pool = torch.empty(nb, 2, 2560, dtype=torch.uint8, device=dev)
+    rng = np.random.default_rng(4)
+    k, v = (rng.standard_normal((1, 2, 40, 128)).astype(np.float16) for _ in range(2))
+    tables = torch.tensor([[nb - 1, nb - 3, nb - 2]], dtype=torch.int32, device=dev)
+    lens = torch.tensor([40], dtype=torch.int32, device=dev)
+    i4.write(torch.from_numpy(k).to(dev), torch.from_numpy(v).to(dev), pool, tables, lens)
+    page_copy.copy_pages([pool], [nb - 2], [nb - 4])
+    tables[0, 2] = nb - 4
+    want = [orc.dequantize(*orc.quantize(x, 32)) for x in (k, v)]
+    for got, x in zip(i4.read(pool, tables, lens, 40), want):
+        assert np.array_equal(got.cpu().numpy(), x.astype(np.float32).astype(np.float16))
+    q = rng.standard_normal((1, 2, 6, 128)).astype(np.float16)
+    got = pd.paged_decode_attention_int4(torch.from_numpy(q).to(dev), pool, tables, lens)
+    small = pool[nb - 4:].cpu().numpy()
+    check(got, q, small, np.array([[3, 1, 0]], np.int32), [40])
 
 
 def test_write_and_read_refusals():

@@ -158,5 +158,11 @@ def test_refusals():
         a = good | bad
         with pytest.raises(ValueError):
             rotary.apply_rotary(a.pop("q"), a.pop("k"), a.pop("cos"), a.pop("sin"), a.pop("positions"), **a)
+    no_q, only_k = rotary.apply_rotary(x[:, :0], x + 1, cos, sin, p)
+    assert no_q.shape == (4, 0, 64)
+    check(only_k, x + 1, cos, sin, p, False)
+    row = torch.ones(1, 1, 64, device="cuda")
+    wide, _ = rotary.apply_rotary(row.expand(4, 2, 64), x, cos, sin, p)              # broadcast inputs
+    check(wide, torch.ones(4, 2, 64, device="cuda"), cos, sin, p, False)
     none, _ = rotary.apply_rotary(x[:0], x[:0], cos, sin, p[:0])
     assert none.shape == (0, 2, 64)
