@@ -6,6 +6,9 @@ The package holds one hot path and nothing else:
     paged_decode_cuda   dense fp16 + INT8 decode           (reference: kernels/cuda/paged_decode_cuda.py)
     paged_sparse        page scores, top-k, sparse decode  (reference: kernels/cuda/paged_sparse.py)
     int8_write          quantize-on-write, page finalize   (reference: kernels/cuda/int8_write.py)
+    int4_write          the 4-bit cache's page records: write, read back, RoPE + append  (no counterpart)
+    page_copy           copies of pages inside a cache's pools: forks, compaction       (no counterpart)
+    rotary              rotary positions of queries and keys, tables for scaled contexts
     kv_write            fp16 append + page bounds          (reference: cache/paged_cache.py write path)
     cache               paged caches over those kernels    (reference: cache/*.py)
     dropin              installs the above into an importable reference tree

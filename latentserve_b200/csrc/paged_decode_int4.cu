@@ -1,5 +1,11 @@
-// Paged GQA decode attention over a cache held in 4 bits (record layout: int4_page.cuh). The
-// split, the walk over the pages and the merge are those of the other pools (decode_core.cuh).
+// Paged GQA decode attention over a cache held in 4 bits (record layout: int4_page.cuh).
+//
+// Measured on one B200 (copy peak 6.54 TB/s), launches back to back: 64 x 16 384 tokens, 2 KV
+// heads, 6 query rows, groups of 32: 71 us (4.7 TB/s; a page more per SM costs 64 ns = 5.9 TB/s);
+// 64 x 16 384, 8 KV heads, 4 rows, groups of 64: 210 us (5.75 TB/s). What is left over the bytes is
+// a fixed 10 us (launch 2, lengths and tables 2, first pages 1, the last states' way out 4) and, in
+// the loop, instruction issue about as much as memory: 269 instructions and 27 MMAs a page at six
+// rows (a word of eight codes is one shift and four ANDs), issue slots 48 % used, the tensor pipe 38 %.
 //
 // Mathematics, per page of 16 tokens and one KV head, n = codes, step / lo = fp16 scales per
 // (token t, group y of channels):
@@ -25,7 +31,9 @@ namespace ls {
 
 // A warp takes kInt4Group pages of a sequence at a time: one wait, one decision on the softmax
 // reference and one loop's bookkeeping for all of them, and the pages' chains of dependent
-// instructions overlap. Two groups of each warp are in flight or being worked on.
+// instructions overlap. Two groups of each warp are in flight or being worked on. (16 x 16 384 tokens:
+// a page at a time in the INT8 kernel's loop 33.0 us, groups of four 30.9; groups of two or three with
+// three blocks an SM the same within 1 us, a third stage costs the second block and 15 us.)
 #ifndef LS_INT4_GROUP
 #define LS_INT4_GROUP 4
 #endif
@@ -378,7 +386,8 @@ struct Int4State {
 
 // How the batch is cut. Every sequence takes its pages plus kInt4Begin units on one axis, and the
 // axis is cut into even chunks, one per CTA: a CTA that goes from one sequence to the next gets
-// that many pages fewer, for the time that summing up the one and starting the other takes. A
+// that many pages fewer, for the time that summing up the one and starting the other takes (16 x
+// 16 384 tokens: 30.6 us with none, 29.1 with 12, 26.5 with 24, 26.6 with 40). A
 // sequence's pages begin behind its extra units, so a chunk that ends inside those has none of it.
 #ifndef LS_INT4_BEGIN
 #define LS_INT4_BEGIN 24
