@@ -45,8 +45,9 @@ struct Int4Fit {
 
 // The quantiser as its formula reads. Out of line: the usual row does not come here.
 template <int G>
-static __device__ __noinline__ Int4Fit int4_fit_divided(const uint4 raw) {
-    const __half2* h2 = reinterpret_cast<const __half2*>(&raw);
+static __device__ __noinline__ Int4Fit int4_fit_divided(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3) {
+    const uint32_t raw[4] = {c0, c1, c2, c3};            // (as words: a uint4 would go through memory)
+    const __half2* h2 = reinterpret_cast<const __half2*>(raw);
     Int4Fit fit;
     float x[8], lo = 65504.f, hi = -65504.f;
 #pragma unroll
@@ -140,7 +141,7 @@ __device__ __forceinline__ Int4Fit int4_fit(const uint4& raw) {
     const bool plain = range <= 131008.f && range * y < 15.4f;
     if (__all_sync(LS_FULL_MASK, plain)) return fit;
 
-    return int4_fit_divided<G>(raw);
+    return int4_fit_divided<G>(raw.x, raw.y, raw.z, raw.w);
 }
 
 // Bytes k of four words next to one another: out[k] = {w0.k, w1.k, w2.k, w3.k}.

@@ -44,28 +44,30 @@ int4_write_kernel(const __half* __restrict__ k, const __half* __restrict__ v, ui
     const int t0 = max(first - page * LS_PAGE, 0), t1 = min(len - page * LS_PAGE, LS_PAGE);
     const __half* src = (warp < 2 ? k + b * sk_b + h * sk_h : v + b * sv_b + h * sv_h) + (lane & 15) * 8;
     const long long st = warp < 2 ? sk_t : sv_t, row0 = (long long)page * LS_PAGE - start;
-    uint4 raw[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int t = page_token(warp, lane, i);
-        raw[i] = make_uint4(0, 0, 0, 0);
-        if (t >= t0 && t < t1) raw[i] = *reinterpret_cast<const uint4*>(src + (row0 + t) * st);
-    }
-    if (blk < 0 || blk >= r.num_blocks) return;          // never write outside the pool
+    const bool there = blk >= 0 && blk < r.num_blocks;   // never write outside the pool
     uint8_t* rec = pool + blk * r.sp_b + h * r.sp_h;
-    if (t0 > 0 || t1 < LS_PAGE) {
-#pragma unroll 1
-        for (int i = 0; i < 4; ++i) {
-            const int t = page_token(warp, lane, i);
-            const Int4Fit fit = int4_fit<G>(i == 0 ? raw[0] : i == 1 ? raw[1] : i == 2 ? raw[2] : raw[3]);
-            const uint32_t bytes = int4_v_bytes(fit.codes, lane & 1);
-            if (t < t0 || t >= t1) continue;
-            if (warp < 2) int4_put_k<G>(rec, t, fit, lane & 15);
-            else int4_put_v<G>(rec, t, fit, bytes, lane & 15);
-        }
+    if (t0 == 0 && t1 == LS_PAGE) {
+        uint4 raw[4];
+        src += (row0 + page_token(warp, lane, 0)) * st;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) raw[i] = *reinterpret_cast<const uint4*>(src + (page_token(warp, 0, i) - page_token(warp, 0, 0)) * st);
+        if (there) int4_put_page<G>(rec, raw, warp, lane);
         return;
     }
-    int4_put_page<G>(rec, raw, warp, lane);
+    if (!there) return;
+#pragma unroll 1
+    for (int i = 0; i < 4; ++i) {
+        const int t = page_token(warp, lane, i);
+        const bool mine = t >= t0 && t < t1;
+        if (!__any_sync(LS_FULL_MASK, mine)) continue;
+        uint4 raw = make_uint4(0, 0, 0, 0);
+        if (mine) raw = *reinterpret_cast<const uint4*>(src + (row0 + t) * st);
+        const Int4Fit fit = int4_fit<G>(raw);
+        const uint32_t bytes = int4_v_bytes(fit.codes, lane & 1);
+        if (!mine) continue;
+        if (warp < 2) int4_put_k<G>(rec, t, fit, lane & 15);
+        else int4_put_v<G>(rec, t, fit, bytes, lane & 15);
+    }
 }
 
 // grid as above for the window [start[b], start[b] + tokens). Rows at or past the sequence's
