@@ -6,9 +6,9 @@
 //
 // Mathematics: int4_page.cuh. A token's K and V row of a head are 512 B of fp16 and 128 + 8 G B of
 // record. Measured on 8 sequences x 8197 tokens x 8 heads, groups of 32: reading back 59 us (5.9
-// TB/s of the measured 6.5; memory bound), writing 91 us (3.9 TB/s): the quantiser's instructions
-// bound it, 588 a warp for eight rows, issue slots 77 % used (both together, with a division per
-// channel and the page put together in shared memory: 412 us; now 149).
+// TB/s of the measured 6.5; memory bound), writing 82 us (4.3 TB/s): the quantiser's instructions
+// bound it, 532 a warp for eight rows, issue slots 80 % used (both together, with a division per
+// channel and the page put together in shared memory: 412 us; now 139).
 #include "int4_page.cuh"
 
 namespace ls {
