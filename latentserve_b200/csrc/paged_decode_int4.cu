@@ -20,8 +20,9 @@
 //
 // Precision: q is scaled by a power of two per row; q, codes, lows are exact in fp16, group sums are
 // split into two fp16 numbers; steps multiply in fp32. The weights w and their products with the V
-// steps are split into high and low fp16 halves, two MMAs per tile: with one fp16 rounding of the
-// product alone, random values of V give outputs 1.4 times as far off as rounding the output is.
+// steps are split into high and low fp16 halves: one fp16 rounding of the product alone (2^-11 of a
+// weight at most, 2e-4 on average, as much as rounding the output) would put outputs of random
+// values 1.4 times as far from the exact ones as they are now.
 // The reference of the online softmax lags by at most 2 (log2), so w <= 4 and w * step <= 4 * 8734,
 // inside fp16 for every step the writer can store.
 #include "decode_core.cuh"
